@@ -15,7 +15,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libeyebrowse_attn.so")
 
-EB_F32, EB_F16, EB_BF16 = 0, 1, 2
+EB_F32, EB_F16, EB_BF16, EB_E4M3, EB_E5M2 = 0, 1, 2, 3, 4
 STATUS = {0: "EB_OK", 1: "EB_ERR_INVALID_ARGUMENT", 2: "EB_ERR_UNSUPPORTED", 3: "EB_ERR_CUDA",
           4: "EB_ERR_WORKSPACE", 5: "EB_ERR_NO_DEVICE", 6: "EB_ERR_DEVICE_TIMEOUT"}
 
@@ -30,7 +30,10 @@ EXPORTS = (
     "eb_workspace_init", "eb_head_concat", "eb_get_device_error",
     "eb_attention_decode_noalloc", "eb_head_broadcast", "eb_linear_f16w",
     "eb_linear_f16w_workspace_bytes", "eb_selftest_wait_timeout",
-    "eb_attention_decode_batched_gather",
+    "eb_attention_decode_batched_gather", "eb_w4_weight_bytes", "eb_w4_pack", "eb_w4_quantize",
+    "eb_linear_w4_workspace_bytes", "eb_linear_w4", "eb_kv8_write",
+    "eb_attention_decode_kv8_workspace_bytes", "eb_attention_decode_kv8",
+    "eb_sample_workspace_bytes", "eb_sample",
 )
 
 
@@ -63,6 +66,26 @@ class AttnLayer(ctypes.Structure):
     _fields_ = [("q_norm_w", ctypes.c_void_p), ("k_norm_w", ctypes.c_void_p),
                 ("v_norm_w", ctypes.c_void_p), ("rope_cos", ctypes.c_void_p),
                 ("rope_sin", ctypes.c_void_p)]
+
+
+class W4(ctypes.Structure):
+    """eb_w4: 4-bit weights with group scales."""
+    _fields_ = [("in_f", ctypes.c_int64), ("out_f", ctypes.c_int64), ("group", ctypes.c_int32),
+                ("dtype_scale", ctypes.c_int32), ("q", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("zero", ctypes.c_void_p)]
+
+
+class Kv8(ctypes.Structure):
+    """eb_kv8: an 8-bit KV cache with block scales."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("batch_stride", ctypes.c_int64),
+                ("scale_batch_stride", ctypes.c_int64), ("block", ctypes.c_int32)]
+
+
+class SampleParams(ctypes.Structure):
+    """eb_sample_params: per-row temperature, top-k, top-p and min-p arrays."""
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p),
+                ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p)]
 
 
 _lib = None
@@ -115,6 +138,23 @@ def lib() -> ctypes.CDLL:
     L.eb_attention_decode_workspace_bytes.restype = _sz
     L.eb_attention_decode_workspace_bytes.argtypes = [dp, _i64, _i64]
     L.eb_attention_decode_noalloc.argtypes = [dp, lp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
+    wp, kp, i32 = ctypes.POINTER(W4), ctypes.POINTER(Kv8), ctypes.c_int32
+    L.eb_w4_weight_bytes.restype = _sz
+    L.eb_w4_weight_bytes.argtypes = [_i64, _i64]
+    L.eb_w4_pack.argtypes = [_vp, _i64, _i64, _vp]
+    L.eb_w4_quantize.argtypes = [_vp, _i64, _i64, i32, i32, _vp, _vp, _vp]
+    L.eb_linear_w4_workspace_bytes.restype = _sz
+    L.eb_linear_w4_workspace_bytes.argtypes = [_i64, _i64, _i64]
+    L.eb_linear_w4.argtypes = [wp, _vp, i32, _i64, _vp, i32, _i64, _i64, _vp, _sz, _vp]
+    L.eb_kv8_write.argtypes = [dp, lp, kp, _i64, _i64, _vp, _vp, _vp]
+    L.eb_attention_decode_kv8_workspace_bytes.restype = _sz
+    L.eb_attention_decode_kv8_workspace_bytes.argtypes = [dp, _i64, _i64]
+    L.eb_attention_decode_kv8.argtypes = [dp, lp, kp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz,
+                                          _vp]
+    L.eb_sample_workspace_bytes.restype = _sz
+    L.eb_sample_workspace_bytes.argtypes = [_i64, _i64]
+    L.eb_sample.argtypes = [_vp, i32, _i64, _i64, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp,
+                            _sz, _vp]
     L.eb_workspace_init.argtypes = [_vp, _sz, _vp]
     L.eb_head_concat.argtypes = [_vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int32, _vp]
     L.eb_get_device_error.argtypes = [ctypes.POINTER(ctypes.c_uint32)]
@@ -201,6 +241,66 @@ def linear_f16w(x, w, y, m, in_f, out_f, workspace=None, stream=None):
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _check(lib().eb_linear_f16w(_ptr(x), _ptr(w), _ptr(y), m, in_f, out_f, _ptr(workspace),
                                 ws_bytes, _stream(stream)), "eb_linear_f16w")
+
+
+# ---------------------------------------------------------------- 4-bit weights
+def w4_weight_bytes(in_f, out_f) -> int:
+    return lib().eb_w4_weight_bytes(in_f, out_f)
+
+
+def w4_pack(codes):
+    """eb_w4_pack (host): codes [out_f, in_f] (numpy uint8, 0..15) -> packed uint8 rows
+    [out_f, ceil(in_f / 128) * 64]."""
+    import numpy as np
+    codes = np.ascontiguousarray(codes, dtype=np.uint8)
+    out_f, in_f = codes.shape
+    q = np.empty((out_f, (in_f + 127) // 128 * 64), np.uint8)
+    _check(lib().eb_w4_pack(codes.ctypes.data, in_f, out_f, q.ctypes.data), "eb_w4_pack")
+    return q
+
+
+def w4_quantize(w, group=128, zero_point=False, dtype_scale=EB_F16):
+    """eb_w4_quantize (host): weights [out_f, in_f] -> (packed rows, scales [groups, out_f],
+    zero points [groups, out_f] or None) as numpy arrays. bf16 scales come back as their uint16
+    bits (numpy has no bf16), f16 scales as float16."""
+    import numpy as np
+    w = np.ascontiguousarray(w, dtype=np.float32)
+    out_f, in_f = w.shape
+    groups = (in_f + group - 1) // group if group > 0 else 0
+    q = np.empty((out_f, (in_f + 127) // 128 * 64), np.uint8)
+    scale = np.empty((groups, out_f), np.uint16)
+    zero = np.empty((groups, out_f), np.uint8) if zero_point else None
+    _check(lib().eb_w4_quantize(w.ctypes.data, in_f, out_f, group, dtype_scale, q.ctypes.data,
+                                scale.ctypes.data, zero.ctypes.data if zero_point else None),
+           "eb_w4_quantize")
+    return q, scale.view(np.float16) if dtype_scale == EB_F16 else scale, zero
+
+
+def make_w4(q, scale, zero, in_f, out_f, group, dtype_scale=None):
+    """eb_w4 over device tensors (kept alive by the object). The scale type is the scale
+    tensor's unless dtype_scale says otherwise."""
+    if dtype_scale is None:
+        dtype_scale = torch_dtype_code(scale.dtype)
+    w = W4(in_f, out_f, group, dtype_scale, _ptr(q), _ptr(scale), _ptr(zero))
+    w._keepalive = (q, scale, zero)
+    return w
+
+
+def linear_w4_workspace_bytes(m, in_f, out_f) -> int:
+    return lib().eb_linear_w4_workspace_bytes(m, in_f, out_f)
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else 0
+
+
+def linear_w4(w: W4, x, y, m, workspace=None, stream=None):
+    """eb_linear_w4: y [m, out_f] = x [m, in_f] @ W^T with 4-bit weights; x and y are tensors in
+    f32, f16 or bf16 whose rows may be strided."""
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().eb_linear_w4(w, _ptr(x), torch_dtype_code(x.dtype), _row_stride(x), _ptr(y),
+                              torch_dtype_code(y.dtype), _row_stride(y), m, _ptr(workspace),
+                              ws_bytes, _stream(stream)), "eb_linear_w4")
 
 
 def rope_tables(max_seq: int, head_dim: int, theta: float, rope_angles: int | None = None):
@@ -339,6 +439,59 @@ def attention_decode_noalloc(desc, layer, pos, q, k, v, kcache, vcache, o, strea
                                              _ptr(q), _ptr(k), _ptr(v), _ptr(kcache),
                                              _ptr(vcache), _ptr(o), _stream(stream)),
            "eb_attention_decode_noalloc")
+
+
+# ---------------------------------------------------------------- 8-bit cache
+def make_kv8(k, v, k_scale, v_scale, block, batch_stride=0, scale_batch_stride=0):
+    """eb_kv8 over device tensors (kept alive by the object): codes [(batch,) max_seq, kv_heads,
+    head_dim] of one byte, scales f32 [(batch,) ceil(max_seq / block), kv_heads]."""
+    c = Kv8(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), batch_stride, scale_batch_stride, block)
+    c._keepalive = (k, v, k_scale, v_scale)
+    return c
+
+
+def kv8_write(desc, layer, cache: Kv8, start, count, k, v, stream=None):
+    """eb_kv8_write: rows [start, start + count) of one sequence's 8-bit cache; layer None writes
+    the rows as they are."""
+    _check(lib().eb_kv8_write(desc, layer, cache, start, count, _ptr(k), _ptr(v),
+                              _stream(stream)), "eb_kv8_write")
+
+
+def attention_decode_kv8_workspace_bytes(desc, batch, max_pos) -> int:
+    return lib().eb_attention_decode_kv8_workspace_bytes(desc, batch, max_pos)
+
+
+def attention_decode_kv8(desc, layer, cache: Kv8, batch, positions, max_pos, q, k, v, o,
+                         workspace=None, stream=None):
+    """eb_attention_decode_kv8: one decode step per sequence over an 8-bit cache; positions None
+    puts every sequence at max_pos, k and v None append nothing."""
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().eb_attention_decode_kv8(desc, layer, cache, batch, _ptr(positions), max_pos,
+                                         _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(workspace),
+                                         ws_bytes, _stream(stream)), "eb_attention_decode_kv8")
+
+
+# ---------------------------------------------------------------- sampling
+def make_sample_params(temperature=None, top_k=None, top_p=None, min_p=None):
+    """eb_sample_params over device arrays of one value per row (f32, top_k int32; None leaves a
+    filter out), kept alive by the object."""
+    p = SampleParams(_ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p))
+    p._keepalive = (temperature, top_k, top_p, min_p)
+    return p
+
+
+def sample_workspace_bytes(rows, vocab) -> int:
+    return lib().eb_sample_workspace_bytes(rows, vocab)
+
+
+def sample(logits, params: SampleParams | None, u, ids, workspace=None, stream=None):
+    """eb_sample: ids [rows] (int32) drawn from logits [rows, vocab] (or one row [vocab]) with the
+    uniform numbers u [rows] (f32)."""
+    rows, vocab = logits.shape if logits.dim() == 2 else (1, logits.shape[0])
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().eb_sample(_ptr(logits), torch_dtype_code(logits.dtype), rows, vocab,
+                           _row_stride(logits), params, _ptr(u), _ptr(ids), _ptr(workspace),
+                           ws_bytes, _stream(stream)), "eb_sample")
 
 
 def workspace_init(workspace, stream=None):

@@ -505,6 +505,73 @@ int eb_linear_f16w(const float* x, const void* w, float* y, int64_t m, int64_t i
                                    reinterpret_cast<cudaStream_t>(stream)));
 }
 
+// Largest sizes the 4-bit calls take: indexes of weights, scales and rows
+// stay inside 64 bits with room, and grids inside their limits.
+static bool w4_sizes_ok(int64_t in_f, int64_t out_f) {
+  return in_f > 0 && out_f > 0 && in_f <= (1 << 24) && out_f <= (1 << 24);
+}
+
+size_t eb_w4_weight_bytes(int64_t in_f, int64_t out_f) {
+  return w4_sizes_ok(in_f, out_f) ? (size_t)out_f * ((size_t)(in_f + 127) / 128) * 64 : 0;
+}
+
+int eb_w4_pack(const uint8_t* codes, int64_t in_f, int64_t out_f, void* q) {
+  if (!codes || !q || !w4_sizes_ok(in_f, out_f)) return EB_ERR_INVALID_ARGUMENT;
+  return w4_pack_host(codes, in_f, out_f, static_cast<uint8_t*>(q));
+}
+
+static bool w4_group_ok(int32_t g) { return g == 32 || g == 64 || g == 128; }
+
+int eb_w4_quantize(const float* w, int64_t in_f, int64_t out_f, int32_t group,
+                   int32_t dtype_scale, void* q, void* scale, uint8_t* zero) {
+  if (!w || !q || !scale || !w4_sizes_ok(in_f, out_f) || !w4_group_ok(group) ||
+      (dtype_scale != EB_F16 && dtype_scale != EB_BF16))
+    return EB_ERR_INVALID_ARGUMENT;
+  return w4_quantize_host(w, in_f, out_f, group, dtype_scale, static_cast<uint8_t*>(q),
+                          static_cast<uint16_t*>(scale), zero);
+}
+
+size_t eb_linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t out_f) {
+  if (m <= 0 || !w4_sizes_ok(in_f, out_f)) return 0;
+  return linear_w4_workspace_bytes(m, in_f, out_f);
+}
+
+int eb_linear_w4(const eb_w4* w, const void* x, int32_t dtype_x, int64_t x_stride, void* y,
+                 int32_t dtype_y, int64_t y_stride, int64_t m, void* workspace,
+                 size_t workspace_bytes, eb_stream_t stream) {
+  if (!w || !w4_sizes_ok(w->in_f, w->out_f) || !w4_group_ok(w->group) ||
+      (w->dtype_scale != EB_F16 && w->dtype_scale != EB_BF16) || !dtype_ok(dtype_x) ||
+      !dtype_ok(dtype_y) || m < 0 || m > (1 << 18))
+    return EB_ERR_INVALID_ARGUMENT;
+  if (x_stride == 0) x_stride = w->in_f;
+  if (y_stride == 0) y_stride = w->out_f;
+  if (x_stride < w->in_f || y_stride < w->out_f) return EB_ERR_INVALID_ARGUMENT;
+  if (m == 0) return EB_OK;
+  if (!x || !y || !w->q || !w->scale || !aligned16(w->q)) return EB_ERR_INVALID_ARGUMENT;
+  if (!device_ok()) return EB_ERR_NO_DEVICE;
+  const size_t need = linear_w4_workspace_bytes(m, w->in_f, w->out_f);
+  if (need > 0 && (!workspace || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return EB_ERR_WORKSPACE;
+  W4Args a{};
+  a.q = w->q;
+  a.scale = w->scale;
+  a.zero = w->zero;
+  a.x = x;
+  a.y = y;
+  a.x_stride = x_stride;
+  a.y_stride = y_stride;
+  a.in_f = w->in_f;
+  a.out_f = w->out_f;
+  a.m = m;
+  a.group = w->group;
+  a.dtype_scale = w->dtype_scale;
+  a.dtype_x = dtype_x;
+  a.dtype_y = dtype_y;
+  a.ws = workspace;
+  return cuda_status(launch_linear_w4(a, reinterpret_cast<cudaStream_t>(stream)));
+}
+
 int eb_attn_decode(const float* q, const float* kcache, const float* vcache, float* o, int64_t h,
                    int64_t hkv, int64_t pos, int64_t hd, int64_t max_seq, float scale,
                    void* workspace, size_t workspace_bytes, eb_stream_t stream) {
@@ -864,6 +931,186 @@ int eb_attention_decode_batched_gather(const eb_attn_desc* d, const eb_attn_laye
   return decode_impl(d, L, batch, positions, 0, max_pos, q, k, v, kcache, vcache,
                      cache_batch_stride, nullptr, qs_of(d), kvs_of(d), 0, workspace,
                      workspace_bytes, reinterpret_cast<cudaStream_t>(stream), &gs, seq_index);
+}
+
+// Shared argument checks of the 8-bit cache calls.
+static int kv8_check(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
+                     int64_t batch) {
+  if (!d || !c) return EB_ERR_INVALID_ARGUMENT;
+  if (d->dtype_cache != EB_E4M3 && d->dtype_cache != EB_E5M2) return EB_ERR_INVALID_ARGUMENT;
+  eb_attn_desc t = *d;
+  t.dtype_cache = EB_F32;  // the other fields are checked as everywhere
+  if (!desc_ok(&t) || d->n_kv_heads > 65535) return EB_ERR_INVALID_ARGUMENT;
+  if (L && (L->rope_cos == nullptr) != (L->rope_sin == nullptr)) return EB_ERR_INVALID_ARGUMENT;
+  if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
+    return EB_ERR_INVALID_ARGUMENT;
+  const int64_t rows = (int64_t)d->max_seq * d->n_kv_heads * d->head_dim;
+  const int64_t blocks = ((int64_t)d->max_seq + c->block - 1) / c->block * d->n_kv_heads;
+  if (c->batch_stride < 0 || c->scale_batch_stride < 0) return EB_ERR_INVALID_ARGUMENT;
+  if (batch > 1 && ((c->batch_stride && c->batch_stride < rows) ||
+                    (c->scale_batch_stride && c->scale_batch_stride < blocks) ||
+                    (c->batch_stride & 15)))
+    return EB_ERR_INVALID_ARGUMENT;
+  return EB_OK;
+}
+static bool kv8_pointers_ok(const eb_kv8* c) {
+  return c->k && c->v && c->k_scale && c->v_scale && aligned16(c->k) && aligned16(c->v);
+}
+static int64_t kv8_bstride(const eb_attn_desc* d, const eb_kv8* c) {
+  return c->batch_stride ? c->batch_stride : (int64_t)d->max_seq * d->n_kv_heads * d->head_dim;
+}
+static int64_t kv8_scale_bstride(const eb_attn_desc* d, const eb_kv8* c) {
+  return c->scale_batch_stride ? c->scale_batch_stride
+                               : ((int64_t)d->max_seq + c->block - 1) / c->block * d->n_kv_heads;
+}
+static Kv8WriteArgs kv8_write_args(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
+                                   const void* k, const void* v) {
+  Kv8WriteArgs w{};
+  w.k = k;
+  w.v = v;
+  w.dtype_kv = d->dtype_qkv;
+  w.kv_stride = w.kv_bstride = kvs_of(d);
+  w.kcache = c->k;
+  w.vcache = c->v;
+  w.k_scale = c->k_scale;
+  w.v_scale = c->v_scale;
+  w.cache_bstride = kv8_bstride(d, c);
+  w.scale_bstride = kv8_scale_bstride(d, c);
+  w.block = c->block;
+  w.hkv = d->n_kv_heads;
+  w.hd = d->head_dim;
+  w.batch = 1;
+  w.e5m2 = d->dtype_cache == EB_E5M2;
+  w.k_norm_w = L ? L->k_norm_w : nullptr;
+  w.v_norm_w = L ? L->v_norm_w : nullptr;
+  w.cos_t = L ? L->rope_cos : nullptr;
+  w.sin_t = L ? L->rope_sin : nullptr;
+  w.eps = d->eps;
+  return w;
+}
+
+int eb_kv8_write(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c, int64_t start,
+                 int64_t count, const void* k, const void* v, eb_stream_t stream) {
+  const int rc = kv8_check(d, L, c, 1);
+  if (rc != EB_OK) return rc;
+  if (start < 0 || count < 0 || start > d->max_seq || count > d->max_seq - start)
+    return EB_ERR_INVALID_ARGUMENT;
+  if (kvs_of(d) < (int64_t)d->n_kv_heads * d->head_dim) return EB_ERR_INVALID_ARGUMENT;
+  if (count == 0) return EB_OK;
+  if (!k || !v || !kv8_pointers_ok(c)) return EB_ERR_INVALID_ARGUMENT;
+  if (!device_ok()) return EB_ERR_NO_DEVICE;
+  Kv8WriteArgs w = kv8_write_args(d, L, c, k, v);
+  w.start = start;
+  w.count = count;
+  return cuda_status(launch_kv8_write(w, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+size_t eb_attention_decode_kv8_workspace_bytes(const eb_attn_desc* d, int64_t batch,
+                                               int64_t max_pos) {
+  eb_kv8 c{};
+  c.block = 16;
+  if (kv8_check(d, nullptr, &c, 1) != EB_OK || batch <= 0 || batch > 32767 || max_pos < 0 ||
+      max_pos >= d->max_seq)
+    return 0;
+  return 0;
+}
+
+int eb_attention_decode_kv8(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
+                            int64_t batch, const int32_t* positions, int64_t max_pos,
+                            const void* q, const void* k, const void* v, void* o,
+                            void* workspace, size_t workspace_bytes, eb_stream_t stream) {
+  const int rc = kv8_check(d, L, c, batch);
+  if (rc != EB_OK) return rc;
+  if (batch < 0 || batch > 32767 || max_pos < 0 || max_pos >= d->max_seq ||
+      (k == nullptr) != (v == nullptr))
+    return EB_ERR_INVALID_ARGUMENT;
+  if (batch > 1 && (qs_of(d) < (int64_t)d->n_heads * d->head_dim ||
+                    os_of(d) < (int64_t)d->n_heads * d->head_dim ||
+                    kvs_of(d) < (int64_t)d->n_kv_heads * d->head_dim))
+    return EB_ERR_INVALID_ARGUMENT;
+  if (batch == 0) return EB_OK;
+  if (!q || !o || !kv8_pointers_ok(c)) return EB_ERR_INVALID_ARGUMENT;
+  if (!device_ok()) return EB_ERR_NO_DEVICE;
+  const size_t need = eb_attention_decode_kv8_workspace_bytes(d, batch, max_pos);
+  if (need > 0 && (!workspace || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return EB_ERR_WORKSPACE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (k) {
+    Kv8WriteArgs w = kv8_write_args(d, L, c, k, v);
+    w.start = max_pos;
+    w.count = 1;
+    w.positions = positions;
+    w.max_pos = (int)max_pos;
+    w.batch = (int)batch;
+    const cudaError_t e = launch_kv8_write(w, st);
+    if (e != cudaSuccess) return cuda_status(e);
+  }
+  Kv8DecodeArgs a{};
+  a.q = q;
+  a.dtype_q = d->dtype_qkv;
+  a.dtype_o = d->dtype_out;
+  a.q_bstride = qs_of(d);
+  a.o_bstride = os_of(d);
+  a.o = o;
+  a.kcache = c->k;
+  a.vcache = c->v;
+  a.k_scale = c->k_scale;
+  a.v_scale = c->v_scale;
+  a.cache_bstride = kv8_bstride(d, c);
+  a.scale_bstride = kv8_scale_bstride(d, c);
+  a.positions = positions;
+  a.max_pos = (int)max_pos;
+  a.window = d->window;
+  a.block = c->block;
+  a.H = d->n_heads;
+  a.hkv = d->n_kv_heads;
+  a.hd = d->head_dim;
+  a.batch = (int)batch;
+  a.max_seq = d->max_seq;
+  a.e5m2 = d->dtype_cache == EB_E5M2;
+  a.q_norm_w = L ? L->q_norm_w : nullptr;
+  a.cos_t = L ? L->rope_cos : nullptr;
+  a.sin_t = L ? L->rope_sin : nullptr;
+  a.eps = d->eps;
+  a.scale_log2 = d->scale * kLog2e;
+  return cuda_status(launch_kv8_decode(a, st));
+}
+
+size_t eb_sample_workspace_bytes(int64_t rows, int64_t vocab) {
+  if (rows <= 0 || vocab <= 0 || vocab > (1 << 24)) return 0;
+  return sample_workspace_bytes(rows, vocab);
+}
+
+int eb_sample(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+              const eb_sample_params* params, const float* u, int32_t* ids, void* workspace,
+              size_t workspace_bytes, eb_stream_t stream) {
+  if (!dtype_ok(dtype) || rows < 0 || rows > (1 << 24) || vocab <= 0 || vocab > (1 << 24))
+    return EB_ERR_INVALID_ARGUMENT;
+  if (row_stride == 0) row_stride = vocab;
+  if (row_stride < vocab) return EB_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return EB_OK;
+  if (!logits || !u || !ids) return EB_ERR_INVALID_ARGUMENT;
+  if (!device_ok()) return EB_ERR_NO_DEVICE;
+  const size_t need = sample_workspace_bytes(rows, vocab);
+  if (need > 0 && (!workspace || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return EB_ERR_WORKSPACE;
+  SampleArgs a{};
+  a.logits = logits;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.row_stride = row_stride;
+  if (params) {
+    a.temperature = params->temperature;
+    a.top_k = params->top_k;
+    a.top_p = params->top_p;
+    a.min_p = params->min_p;
+  }
+  a.u = u;
+  a.ids = ids;
+  return cuda_status(launch_sample(a, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 int eb_workspace_init(void* workspace, size_t workspace_bytes, eb_stream_t stream) {

@@ -136,6 +136,84 @@ cudaError_t launch_linear(const float* x, const void* w, float* y, int64_t m, in
                           int64_t out_f, void* ws, LinearPath path, unsigned* err,
                           cudaStream_t st);
 
+// ------------------------------------------------------------- linear_w4 (eb_w4.cu)
+struct W4Args {
+  const void* q;          // packed codes (eb_w4)
+  const void* scale;      // [groups][out_f], dtype_scale
+  const uint8_t* zero;    // [groups][out_f] or nullptr (8)
+  const void* x;
+  void* y;
+  int64_t x_stride, y_stride;
+  int64_t in_f, out_f, m;
+  int group, dtype_scale, dtype_x, dtype_y;
+  void* ws;
+};
+size_t linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t out_f);
+cudaError_t launch_linear_w4(const W4Args& a, cudaStream_t st);
+int w4_pack_host(const uint8_t* codes, int64_t in_f, int64_t out_f, uint8_t* q);
+int w4_quantize_host(const float* w, int64_t in_f, int64_t out_f, int group, int dtype_scale,
+                     uint8_t* q, uint16_t* scale, uint8_t* zero);
+
+// ------------------------------------------------------------- 8-bit cache (eb_kv8.cu)
+struct Kv8WriteArgs {
+  const void* k;
+  const void* v;
+  int dtype_kv;
+  int64_t kv_stride, kv_bstride;  // elements between rows, between sequences
+  void* kcache;
+  void* vcache;
+  float* k_scale;
+  float* v_scale;
+  int64_t cache_bstride, scale_bstride;
+  int64_t start, count;      // cache rows [start, start + count)
+  const int32_t* positions;  // per sequence instead of start (count 1), or nullptr
+  int max_pos;               // positions outside [0, max_pos] are skipped
+  int block, hkv, hd, batch;
+  bool e5m2;
+  const float* k_norm_w;
+  const float* v_norm_w;
+  const float* cos_t;
+  const float* sin_t;
+  float eps;
+};
+cudaError_t launch_kv8_write(const Kv8WriteArgs& a, cudaStream_t st);
+
+struct Kv8DecodeArgs {
+  const void* q;
+  int dtype_q, dtype_o;
+  int64_t q_bstride, o_bstride;
+  void* o;
+  const void* kcache;
+  const void* vcache;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t cache_bstride, scale_bstride;
+  const int32_t* positions;  // or nullptr: every sequence at max_pos
+  int max_pos, window;
+  int block, H, hkv, hd, batch, max_seq;
+  bool e5m2;
+  const float* q_norm_w;
+  const float* cos_t;
+  const float* sin_t;
+  float eps, scale_log2;
+};
+cudaError_t launch_kv8_decode(const Kv8DecodeArgs& a, cudaStream_t st);
+
+// ------------------------------------------------------------- sampling (eb_sample.cu)
+struct SampleArgs {
+  const void* logits;
+  int dtype;
+  int64_t rows, vocab, row_stride;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* u;
+  int32_t* ids;
+};
+size_t sample_workspace_bytes(int64_t rows, int64_t vocab);
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st);
+
 // Latency decode for f32/bf16 caches (eb_decode_cl.cu): n_chunks (1..16)
 // CTAs per (sequence, KV-head group) form a cluster and merge through
 // distributed shared memory; no workspace. a.chunk = rows per CTA.

@@ -1,0 +1,169 @@
+// eb_kv8.cu -- the 8-bit KV cache: rows in (prompt pieces and decode steps) and
+// decode attention for any head_dim.
+//
+// A block of `block` rows of one KV head shares a power-of-two scale for K and
+// one for V. A write finds the largest magnitude of its rows in a block, takes
+// the larger of the scale that needs and the block's own, and rounds: the new
+// rows once, the block's earlier rows again where the scale grew.
+#include "eb_kv8.cuh"
+#include "eb_rowops.cuh"
+
+namespace eb {
+
+// One CTA per (block of rows, KV head, K or V of a sequence), rows staged as
+// f32 in shared memory.
+__global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
+  extern __shared__ float rows[];
+  __shared__ float warp_max_[8];
+  const int which = blockIdx.z & 1, b = blockIdx.z >> 1, head = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t start = a.start;
+  if (a.positions) {
+    const int p = a.positions[b];
+    if (p < 0 || p > a.max_pos) return;  // an empty slot of the batch
+    start = p;
+  }
+  const int64_t end = start + a.count;
+  const int64_t blk = start / a.block + blockIdx.x;
+  const int64_t lo = max(start, blk * a.block), hi = min(end, (blk + 1) * a.block);
+  const int n = (int)(hi - lo), hd = a.hd;
+
+  const void* src = which ? a.v : a.k;
+  float amax = 0.f;
+  for (int r = warp; r < n; r += 8) {
+    float* row = rows + r * hd;
+    const int64_t t = lo + r;
+    const int64_t at = b * a.kv_bstride + (t - start) * a.kv_stride + (int64_t)head * hd;
+    for (int d = lane; d < hd; d += 32) row[d] = ld_any(src, at + d, a.dtype_kv);
+    __syncwarp();
+    warp_row_norm(row, hd, which ? a.v_norm_w : a.k_norm_w, a.eps, lane);
+    if (!which && a.cos_t)
+      warp_row_rope(row, hd, a.cos_t + t * (hd / 2), a.sin_t + t * (hd / 2), lane);
+    for (int d = lane; d < hd; d += 32) amax = f8_amax(amax, row[d]);
+  }
+  amax = warp_max(amax);
+  if (lane == 0) warp_max_[warp] = amax;
+  __syncthreads();
+  for (int i = 0; i < 8; i++) amax = fmaxf(amax, warp_max_[i]);
+
+  float* scale = (which ? a.v_scale : a.k_scale) + b * a.scale_bstride + blk * a.hkv + head;
+  const int64_t stride = (int64_t)a.hkv * hd;
+  uint8_t* cache = static_cast<uint8_t*>(which ? a.vcache : a.kcache) + b * a.cache_bstride +
+                   (int64_t)head * hd;
+  float s = f8_need_scale(amax, a.e5m2);
+  const int before = (int)(lo - blk * a.block);  // rows of the block in front of the new ones
+  if (before > 0) {
+    const float old = *scale;
+    __syncthreads();  // every thread has read the old scale before it is replaced
+    s = fmaxf(s, old);
+    if (s != old) {
+      const float ratio = old / s;
+      uint8_t* c = cache + blk * a.block * stride;
+      for (int i = threadIdx.x; i < before * hd; i += 256) {
+        uint8_t* p = c + (int64_t)(i / hd) * stride + i % hd;
+        *p = f8_encode(f8_decode(*p, a.e5m2) * ratio, a.e5m2);
+      }
+    }
+  }
+  if (threadIdx.x == 0) *scale = s;
+  const float inv = 1.0f / s;
+  for (int i = threadIdx.x; i < n * hd; i += 256)
+    cache[(lo + i / hd) * stride + i % hd] = f8_encode(rows[i] * inv, a.e5m2);
+}
+
+cudaError_t launch_kv8_write(const Kv8WriteArgs& a, cudaStream_t st) {
+  const int64_t per = a.positions ? 1 : (a.start + a.count - 1) / a.block - a.start / a.block + 1;
+  const int rows = (int)(a.count < a.block ? a.count : a.block);
+  const size_t smem = (size_t)rows * a.hd * sizeof(float);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        kv8_write_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * 4);
+    if (e != cudaSuccess) return e;
+  }
+  dim3 grid((unsigned)per, a.hkv, 2 * a.batch);
+  kv8_write_kernel<<<grid, 256, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+// Decode attention for any even head_dim up to 256: one CTA per (sequence,
+// query head), a warp per key row, an online softmax per warp.
+constexpr int kSimtWarps = 8;
+__global__ void __launch_bounds__(kSimtWarps * 32) kv8_decode_simt_kernel(Kv8DecodeArgs a) {
+  __shared__ float q[256];
+  __shared__ float acc_s[kSimtWarps][256];
+  __shared__ float m_s[kSimtWarps], l_s[kSimtWarps];
+  const int h = blockIdx.x, b = blockIdx.y, hd = a.hd;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pos = a.positions ? a.positions[b] : a.max_pos;
+  if (pos < 0 || pos > a.max_pos) return;
+  const int kvh = h / (a.H / a.hkv);
+  if (warp == 0) {
+    const int64_t at = b * a.q_bstride + (int64_t)h * hd;
+    for (int d = lane; d < hd; d += 32) q[d] = ld_any(a.q, at + d, a.dtype_q);
+    __syncwarp();
+    warp_row_norm(q, hd, a.q_norm_w, a.eps, lane);
+    if (a.cos_t)
+      warp_row_rope(q, hd, a.cos_t + (int64_t)pos * (hd / 2), a.sin_t + (int64_t)pos * (hd / 2),
+                    lane);
+  }
+  __syncthreads();
+  float qr[8], acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    qr[j] = lane + 32 * j < hd ? q[lane + 32 * j] * a.scale_log2 : 0.f;
+    acc[j] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const uint8_t* kc = static_cast<const uint8_t*>(a.kcache) + b * a.cache_bstride;
+  const uint8_t* vc = static_cast<const uint8_t*>(a.vcache) + b * a.cache_bstride;
+  const float* ks = a.k_scale + b * a.scale_bstride + kvh;
+  const float* vs = a.v_scale + b * a.scale_bstride + kvh;
+  const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  for (int t = row_lo + warp; t <= pos; t += kSimtWarps) {
+    const int64_t at = ((int64_t)t * a.hkv + kvh) * hd;
+    const int64_t sb = (int64_t)(t / a.block) * a.hkv;
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (lane + 32 * j < hd) dot = fmaf(qr[j], f8_decode(kc[at + lane + 32 * j], a.e5m2), dot);
+    const float x = warp_sum(dot) * ks[sb];
+    const float mn = fmaxf(m, x);
+    const float corr = m == -INFINITY ? 0.f : exp2f(m - mn);
+    const float p = exp2f(x - mn);
+    l = l * corr + p;
+    const float pv = p * vs[sb];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (lane + 32 * j < hd)
+        acc[j] = fmaf(pv, f8_decode(vc[at + lane + 32 * j], a.e5m2), acc[j] * corr);
+    m = mn;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    if (lane + 32 * j < hd) acc_s[warp][lane + 32 * j] = acc[j];
+  if (lane == 0) {
+    m_s[warp] = m;
+    l_s[warp] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY, L = 0.f, w[kSimtWarps];
+  for (int i = 0; i < kSimtWarps; i++)
+    if (l_s[i] != 0.f) M = fmaxf(M, m_s[i]);
+  for (int i = 0; i < kSimtWarps; i++) {
+    w[i] = l_s[i] != 0.f ? exp2f(m_s[i] - M) : 0.f;
+    L += l_s[i] * w[i];
+  }
+  for (int d = threadIdx.x; d < hd; d += kSimtWarps * 32) {
+    float o = 0.f;
+    for (int i = 0; i < kSimtWarps; i++)
+      if (l_s[i] != 0.f) o += acc_s[i][d] * w[i];
+    st_any(a.o, b * a.o_bstride + (int64_t)h * hd + d, a.dtype_o, o / L);
+  }
+}
+
+cudaError_t launch_kv8_decode(const Kv8DecodeArgs& a, cudaStream_t st) {
+  kv8_decode_simt_kernel<<<dim3(a.H, a.batch), kSimtWarps * 32, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace eb

@@ -45,7 +45,8 @@ typedef enum {
   EB_ERR_DEVICE_TIMEOUT = 6    /* a kernel's bounded wait gave up (see eb_get_device_error) */
 } eb_status;
 
-typedef enum { EB_F32 = 0, EB_F16 = 1, EB_BF16 = 2 } eb_dtype;
+/* The 8-bit types are cache types of the kv8 calls only. */
+typedef enum { EB_F32 = 0, EB_F16 = 1, EB_BF16 = 2, EB_E4M3 = 3, EB_E5M2 = 4 } eb_dtype;
 
 /* Human-readable name of a status code. */
 EB_API const char* eb_status_string(int status);
@@ -318,6 +319,149 @@ EB_API int eb_head_concat(const void* src, void* dst, int64_t shards, int64_t ro
 EB_API int eb_head_broadcast(const void* local, void* multicast, int64_t rows,
                              int64_t n_heads_total, int32_t head_offset, int32_t n_heads,
                              int64_t head_dim, int32_t dtype, eb_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * A decode step with fewer bytes: 4-bit projection weights, an 8-bit KV cache
+ * and the draw of the next token on the GPU. No reference counterparts: the
+ * reference keeps f16 weights and an f32 cache and takes the argmax.
+ * ------------------------------------------------------------------------ */
+
+/* 4-bit weights with one scale per group of consecutive inputs:
+ *   W[o, i] = scale[i / group, o] * (code[o, i] - zero[i / group, o]),
+ * codes and zero points 0..15, the zero point 8 where `zero` is NULL.
+ *   q:     DEVICE, 16-byte aligned, eb_w4_weight_bytes(in_f, out_f) bytes. A
+ *          row is cut into blocks of 128 inputs of 64 bytes; byte
+ *          16 c + 4 i + b of a block holds inputs 32 i + 8 c + 2 b (low
+ *          nibble) and 32 i + 8 c + 2 b + 1 (high nibble). Inputs past in_f
+ *          hold 0. (Four neighbouring threads' 16-byte loads then hold whole
+ *          groups of 32 inputs between them.)
+ *   scale: DEVICE [ceil(in_f / group), out_f] in dtype_scale
+ *   zero:  DEVICE [ceil(in_f / group), out_f] bytes, or NULL */
+typedef struct {
+  int64_t in_f, out_f; /* any sizes; the last group and the last block may be short */
+  int32_t group;       /* 32, 64 or 128 */
+  int32_t dtype_scale; /* EB_F16 or EB_BF16 */
+  const void* q;
+  const void* scale;
+  const uint8_t* zero;
+} eb_w4;
+
+/* Bytes of the packed codes: out_f * ceil(in_f / 128) * 64. 0 for sizes < 1. */
+EB_API size_t eb_w4_weight_bytes(int64_t in_f, int64_t out_f);
+
+/* Host functions (no device work, all arrays HOST), run once when a model is
+ * loaded, like eb_rope_tables.
+ * eb_w4_pack: codes [out_f, in_f] (one per byte, 0..15; more is refused) into
+ * the packed layout.
+ * eb_w4_quantize: w [out_f, in_f] f32 into packed codes and scales. zero ==
+ * NULL: scale = max|w| / 7 over the group, code = 8 + w / scale. zero != NULL:
+ * lo = min(w, 0), hi = max(w, 0), scale = (hi - lo) / 15, zero = -lo / scale,
+ * code = zero + w / scale. Every quotient is of f64 values and rounded to
+ * nearest, ties to even, after the scale was rounded to dtype_scale; codes
+ * and zero points are clamped to 0..15. A group whose scale rounds to zero
+ * holds zeros. A weight that is not finite, or whose scale passes
+ * dtype_scale's range, is refused with EB_ERR_INVALID_ARGUMENT. */
+EB_API int eb_w4_pack(const uint8_t* codes, int64_t in_f, int64_t out_f, void* q);
+EB_API int eb_w4_quantize(const float* w, int64_t in_f, int64_t out_f, int32_t group,
+                          int32_t dtype_scale, void* q, void* scale, uint8_t* zero);
+
+/* y [m, out_f] = x [m, in_f] * W^T, beside eb_linear_f16w. x and y in f32, f16
+ * or bf16, rows x_stride / y_stride elements apart (0 = in_f / out_f). Every
+ * product is formed exactly and summed in f32, whatever the types (f32
+ * activations are split into three bf16 parts that add up to them); a row
+ * with a value that is not finite yields NaN or an infinity. Made for the
+ * few rows of decode steps: up to 64 rows stream the weights from memory
+ * once, each further 64 rows once more (from L2 where they fit).
+ * eb_linear_w4_workspace_bytes is 0 for m <= 8. The workspace is 256-byte
+ * aligned and needs no initialisation. */
+EB_API size_t eb_linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t out_f);
+EB_API int eb_linear_w4(const eb_w4* w, const void* x, int32_t dtype_x, int64_t x_stride, void* y,
+                        int32_t dtype_y, int64_t y_stride, int64_t m, void* workspace,
+                        size_t workspace_bytes, eb_stream_t stream);
+
+/* An 8-bit KV cache: codes in desc->dtype_cache (EB_E4M3 or EB_E5M2) and one
+ * f32 scale per (block of rows, KV head), for K and for V; the value of a
+ * code is code * scale.
+ *   k, v:             [max_seq, n_kv_heads, head_dim] bytes, 16-byte aligned
+ *   k_scale, v_scale: [ceil(max_seq / block), n_kv_heads] f32
+ * Calls that write choose the scale: the smallest power of two (2^-64 at
+ * least) at which no finite value of the new rows passes the type's largest
+ * (448 for E4M3, 57344 for E5M2), or the block's present scale if that is
+ * larger. Where rows before the new ones in the block were written at a
+ * smaller scale they are rounded again at the new one, which is exact but
+ * for values that become subnormal. A write of a block's first row starts
+ * the block anew, whatever it held. Values round to nearest, ties to even;
+ * an infinity is stored as the type's largest value, a NaN as NaN. Rows
+ * behind the written ones are left as they are. Calls that only read take
+ * any positive scales. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t batch_stride;       /* bytes between sequences' k (and v); 0 = dense. A multiple of 16 */
+  int64_t scale_batch_stride; /* floats between sequences' k_scale (and v_scale); 0 = dense */
+  int32_t block;              /* rows per scale: 16, 32, 64 or 128 */
+} eb_kv8;
+
+/* A prompt's (or a piece's) rows into one sequence's 8-bit cache: k ->
+ * RMSNorm -> RoPE (table row start + r), v -> RMSNorm, as
+ * eb_attention_prefill_kv, then rows [start, start + count) of the cache and
+ * their scales. layer may be NULL (rows that are prepared already, e.g. the
+ * rows of the cache that eb_attention_prefill wrote). k and v rows are
+ * kv_stride elements apart, in dtype_qkv. */
+EB_API int eb_kv8_write(const eb_attn_desc* desc, const eb_attn_layer* layer, const eb_kv8* cache,
+                        int64_t start, int64_t count, const void* k, const void* v,
+                        eb_stream_t stream);
+
+/* eb_attention_decode_batched over an 8-bit cache: appends each sequence's new
+ * k and v rows at positions[b] (k == v == NULL appends nothing) and attends
+ * rows 0..=positions[b] (the last `window` of them) into o, in f32
+ * arithmetic throughout. positions: DEVICE int32; a value outside [0,
+ * max_pos] marks an empty slot of the batch, whose cache and output rows are
+ * left as they are. positions == NULL: every sequence is at max_pos. Row
+ * strides as for eb_attention_decode_batched; no alignment beyond the
+ * element's for q, k, v and o. A workspace smaller than
+ * eb_attention_decode_kv8_workspace_bytes is refused; it is zeroed once by
+ * eb_workspace_init, each call leaves its counters at zero, and calls that
+ * share one must not overlap on the GPU. */
+EB_API size_t eb_attention_decode_kv8_workspace_bytes(const eb_attn_desc* desc, int64_t batch,
+                                                      int64_t max_pos);
+EB_API int eb_attention_decode_kv8(const eb_attn_desc* desc, const eb_attn_layer* layer,
+                                   const eb_kv8* cache, int64_t batch, const int32_t* positions,
+                                   int64_t max_pos, const void* q, const void* k, const void* v,
+                                   void* o, void* workspace, size_t workspace_bytes,
+                                   eb_stream_t stream);
+
+/* How eb_sample draws, per row (DEVICE arrays of `rows` values; a NULL array
+ * leaves its filter out, temperature NULL = 1). */
+typedef struct {
+  const float* temperature; /* <= 0 or NaN: greedy, the largest logit, the first of equals */
+  const int32_t* top_k;     /* < 1: off */
+  const float* top_p;       /* >= 1 or NaN: off; <= 0: one token */
+  const float* min_p;       /* <= 0 or NaN: off */
+} eb_sample_params;
+
+/* One token id per row of logits [rows, vocab] (f32, f16 or bf16, rows
+ * row_stride elements apart, 0 = vocab), drawn with the given uniform numbers
+ * u [rows] in [0, 1). With the weight exp((logit - max) / temperature), and
+ * tokens ordered by logit, the first of equals before the others:
+ *   top_k keeps the first top_k tokens;
+ *   top_p keeps, of those, each token before which less than top_p of their
+ *   weight stands (so at least one);
+ *   min_p keeps, of those, the weights of at least min_p, and the largest.
+ * The id is the first, in the vocabulary's order, at which the running sum of
+ * the kept weights passes u times their total. Weights and sums are in f64,
+ * so that the draw does not hang on rounding; results do not depend on
+ * timing. Weights below 2^-60 count as zero (u has 24 bits) and are never
+ * drawn. A NaN logit counts as -infinity, several +infinity as equals that
+ * leave no weight to others. A row without a logit above -infinity gives -1.
+ * u is clamped to [0, 1 - 2^-24], NaN to 0.
+ * ids: DEVICE int32 [rows]. vocab <= 2^24. */
+EB_API size_t eb_sample_workspace_bytes(int64_t rows, int64_t vocab);
+EB_API int eb_sample(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
+                     int64_t row_stride, const eb_sample_params* params, const float* u,
+                     int32_t* ids, void* workspace, size_t workspace_bytes, eb_stream_t stream);
 
 /* Returns and clears the device-side error word of the current device: a
  * non-zero value means some kernel's bounded wait gave up (the kernel then
