@@ -13,6 +13,19 @@ namespace eb {
 // buffers, this GPU's and its peers'.
 constexpr int kMaxGather = 8;
 
+// Lets `kern` use `bytes` of dynamic shared memory on the current device: one
+// runtime call per kernel and device, remembered in *configured.
+template <typename K>
+inline cudaError_t allow_smem(K* kern, int bytes, unsigned* configured) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 32 && (__atomic_load_n(configured, __ATOMIC_ACQUIRE) & (1u << dev))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 32) __atomic_fetch_or(configured, 1u << dev, __ATOMIC_RELEASE);
+  return e;
+}
+
 // ------------------------------------------------------------- small kernels
 cudaError_t launch_rope(const float* x, const float* cos_t, const float* sin_t, float* out,
                         int64_t seq, int64_t n_heads, int64_t hd, int64_t base_pos,

@@ -366,14 +366,15 @@ EB_API int eb_w4_quantize(const float* w, int64_t in_f, int64_t out_f, int32_t g
                           int32_t dtype_scale, void* q, void* scale, uint8_t* zero);
 
 /* y [m, out_f] = x [m, in_f] * W^T, beside eb_linear_f16w. x and y in f32, f16
- * or bf16, rows x_stride / y_stride elements apart (0 = in_f / out_f). Every
- * product is formed exactly and summed in f32, whatever the types (f32
- * activations are split into three bf16 parts that add up to them); a row
- * with a value that is not finite yields NaN or an infinity. Made for the
- * few rows of decode steps: up to 64 rows stream the weights from memory
- * once, each further 64 rows once more (from L2 where they fit).
- * eb_linear_w4_workspace_bytes is 0 for m <= 8. The workspace is 256-byte
- * aligned and needs no initialisation. */
+ * or bf16, rows x_stride / y_stride elements apart (0 = in_f / out_f); x and y
+ * do not overlap. Sums are in f32; 16-bit activations enter exactly, f32 ones
+ * with 22 bits (and both without what lies below 2^-39 of the largest of 128
+ * neighbouring inputs); a row with a value that is not finite yields NaN or
+ * an infinity. Made for the few rows of decode steps: up to 24 rows of 16-bit
+ * activations, or 12 of f32, stream the weights once, more rows once more for
+ * each such number (from L2 where they fit). m <= 2^18, in_f and out_f <=
+ * 2^24. eb_linear_w4_workspace_bytes is 0 for m <= 8. The workspace is
+ * 256-byte aligned and needs no initialisation. */
 EB_API size_t eb_linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t out_f);
 EB_API int eb_linear_w4(const eb_w4* w, const void* x, int32_t dtype_x, int64_t x_stride, void* y,
                         int32_t dtype_y, int64_t y_stride, int64_t m, void* workspace,

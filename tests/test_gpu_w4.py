@@ -58,6 +58,19 @@ def test_sizes(eb, in_f, out_f, m):
     assert eb.device_error() == 0
 
 
+@pytest.mark.parametrize("m,in_f,out_f", [(8, 2304, 19000), (8, 14336, 4096), (1, 14336, 4096), (24, 5000, 9000)])
+def test_long_rows(eb, m, in_f, out_f):
+    """Rows whose inputs are staged in several pieces, over row counts that split them differently."""
+    import torch
+    w4, _ = _make(eb, in_f, out_f, 128, True, "f16", in_f)
+    x = torch.randn(m, in_f, generator=torch.Generator().manual_seed(m)).cuda()
+    codes = torch.from_numpy(qo.w4_unpack(w4._keepalive[0].cpu().numpy(), in_f)).cuda()
+    g = torch.arange(in_f, device="cuda") // 128
+    scale, zero = w4._keepalive[1], w4._keepalive[2]
+    W = (codes.double() - zero[g].T.double()) * scale[g].T.double()
+    _check(_call(eb, w4, x, "f32", m, out_f), (x.double() @ W.T).cpu().numpy(), in_f, "f32")
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("zero", [False, True])
 @pytest.mark.parametrize("x_dtype,y_dtype,s_dtype", [("f32", "f32", "bf16"), ("f16", "f16", "f16"),
