@@ -1005,14 +1005,45 @@ int eb_kv8_write(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
   return cuda_status(launch_kv8_write(w, reinterpret_cast<cudaStream_t>(stream)));
 }
 
+// Split of the contexts of an 8-bit decode call into chunks of whole 128-row
+// tiles: about as many CTAs as the SMs hold at once (two each at head_dim 128,
+// one at 256), chunks of at most 64 tiles so that unequal contexts even out,
+// at most 256 of them.
+struct Kv8Plan {
+  int gsubs, chunk, cmax;
+  int64_t bound;  // chunks of any context up to max_pos, never fewer for a larger one
+};
+static Kv8Plan plan_kv8(const eb_attn_desc* d, int64_t batch, int64_t max_pos) {
+  Kv8Plan p{};
+  p.gsubs = (d->n_heads / d->n_kv_heads + 7) / 8;
+  // a window may begin inside a tile
+  const int64_t tiles = std::min<int64_t>(
+      max_pos / 128 + 1, d->window > 0 ? ((int64_t)d->window + 126) / 128 + 1 : INT64_MAX);
+  const int64_t n = batch * d->n_kv_heads * p.gsubs;
+  const int64_t target = (d->head_dim == 128 ? 2 : 1) * (int64_t)sm_count();
+  int64_t c = std::min<int64_t>((tiles * n + target - 1) / target, 64);
+  c = std::max<int64_t>(c, (tiles + 255) / 256);
+  p.chunk = (int)c * 128;
+  p.cmax = (int)((tiles + c - 1) / c);
+  p.bound = std::min(std::min<int64_t>(tiles, 256),
+                     std::max((target + n - 1) / n, (tiles + 63) / 64));
+  return p;
+}
+static DecodePlan kv8_layout(const eb_attn_desc* d, int64_t batch, int64_t chunks) {
+  DecodePlan w{};
+  w.cmax = (int)chunks;
+  if (chunks > 1) decode_layout(w, batch, d->n_heads, d->head_dim);
+  return w;
+}
+
 size_t eb_attention_decode_kv8_workspace_bytes(const eb_attn_desc* d, int64_t batch,
                                                int64_t max_pos) {
   eb_kv8 c{};
   c.block = 16;
   if (kv8_check(d, nullptr, &c, 1) != EB_OK || batch <= 0 || batch > 32767 || max_pos < 0 ||
-      max_pos >= d->max_seq)
+      max_pos >= d->max_seq || !kv8_tc_supported(d->head_dim))
     return 0;
-  return 0;
+  return kv8_layout(d, batch, plan_kv8(d, batch, max_pos).bound).bytes;
 }
 
 int eb_attention_decode_kv8(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
@@ -1074,7 +1105,21 @@ int eb_attention_decode_kv8(const eb_attn_desc* d, const eb_attn_layer* L, const
   a.sin_t = L ? L->rope_sin : nullptr;
   a.eps = d->eps;
   a.scale_log2 = d->scale * kLog2e;
-  return cuda_status(launch_kv8_decode(a, st));
+  if (!kv8_tc_supported(d->head_dim)) return cuda_status(launch_kv8_decode(a, st));
+  const Kv8Plan p = plan_kv8(d, batch, max_pos);
+  const DecodePlan w = kv8_layout(d, batch, p.cmax);
+  a.gsubs = p.gsubs;
+  a.chunk = p.chunk;
+  a.cmax = p.cmax;
+  if (p.cmax > 1) {
+    char* base = static_cast<char*>(workspace);
+    a.ws_cnt = reinterpret_cast<unsigned*>(base + w.cnt_off);
+    a.ws_ml = reinterpret_cast<float*>(base + w.ml_off);
+    a.ws_acc = reinterpret_cast<float*>(base + w.acc_off);
+  }
+  a.err = error_word_ptr();
+  if (!a.err) return EB_ERR_CUDA;
+  return cuda_status(launch_kv8_decode_tc(a, st));
 }
 
 size_t eb_sample_workspace_bytes(int64_t rows, int64_t vocab) {

@@ -209,8 +209,19 @@ struct Kv8DecodeArgs {
   const float* cos_t;
   const float* sin_t;
   float eps, scale_log2;
+  // tensor-core kernel: head groups per KV head, rows per chunk (a multiple of
+  // 128), chunks of the longest context, split-K workspace
+  int gsubs, chunk, cmax;
+  unsigned* ws_cnt;  // [B][hkv * gsubs] tickets
+  float* ws_ml;      // [B][H][cmax] x (m, l)
+  float* ws_acc;     // [B][H][cmax][hd]
+  unsigned* err;
 };
+// Any even head_dim up to 256.
 cudaError_t launch_kv8_decode(const Kv8DecodeArgs& a, cudaStream_t st);
+// head_dim 128 and 256 (eb_kv8_tc.cu).
+bool kv8_tc_supported(int hd);
+cudaError_t launch_kv8_decode_tc(const Kv8DecodeArgs& a, cudaStream_t st);
 
 // ------------------------------------------------------------- sampling (eb_sample.cu)
 struct SampleArgs {
