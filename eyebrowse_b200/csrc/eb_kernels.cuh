@@ -234,6 +234,7 @@ struct SampleArgs {
   const float* min_p;
   const float* u;
   int32_t* ids;
+  int cluster;  // CTAs per row, set by the launcher
 };
 size_t sample_workspace_bytes(int64_t rows, int64_t vocab);
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st);

@@ -4,154 +4,666 @@
 // Tokens are ordered by (logit descending, index ascending): every filter
 // keeps a prefix of that order. A composite key, the logit's ordered bits
 // above the complemented index, turns the order into one of distinct 64-bit
-// integers, so a prefix is {key >= cut}.
+// integers, so a prefix is {key >= cut}; the token is then found by a running
+// sum in index order over the kept ones. Nothing is sorted but a list of at
+// most kCap tokens around the cut:
+//
+//   pass 1  the largest logit M (with no filter: the sums too, and pass 4)
+//   pass 2  a histogram of (M - logit) / T in 1/32 octaves of weight, counts
+//           only. Where it shows that top_k's cut, or all that top_p's can
+//           need, lies within kCap tokens, the window is those bins from the
+//           top; else the bins around the estimated cut.
+//   pass 3  the window's tokens into the list; above it, and in all for top_p,
+//           the weights' exact sums. The list is sorted and the cut found
+//           among exact sums. A cut outside the window, or a bin of more than
+//           kCap tokens at the cut, is left to a bisection over the keys with
+//           a pass per bit: exact for any input, and slow.
+//   pass 4  sums of the kept weights, a run of the row per warp; the run in
+//           which u's share falls is then walked by its CTA. With all kept
+//           tokens in the list, the list sorted by index takes its place.
+//
+// Weights are f64 (2^t by a 16-entry table and a Taylor polynomial of degree
+// 5: 2 * 10^-13 relative): in f32 the running sum over a vocabulary would be
+// off by more than many a token's share. Sums meet in a fixed order, so
+// results do not depend on timing (the list's order of arrival is undone by
+// the sort).
+//
+// A row is shared by a cluster of 1 to 8 CTAs; passes after the first read it
+// from L1 or L2. What bounds it: for many open rows the f64 pipe (12
+// operations a token), for one row the chain of cluster barriers.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "eb_common.cuh"
 #include "eb_kernels.cuh"
 #include "eb_rowops.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace eb {
 
-constexpr int kSampleThreads = 1024;
+constexpr int kSampleWarps = 16, kSampleThreads = kSampleWarps * 32;
+constexpr int kMaxCluster = 8;
+constexpr int kCap = 2048;
+constexpr int kOctaves = 60, kPerOctave = 32, kBins = kOctaves * kPerOctave;
+typedef unsigned long long u64;
 
-// Floats as unsigned integers of the same order.
+struct SampleShared {
+  u64 list[kCap];
+  double tab[16];
+  double seg[kMaxCluster * kSampleWarps];  // sums of the row's runs
+  float seg_ref[kMaxCluster * kSampleWarps];
+  double part[2][2][kMaxCluster];  // CTAs' sums, by turn
+  double warp_d[kSampleWarps];
+  u64 warp_best[kSampleWarps];
+  u64 best[kMaxCluster];
+  u64 cut;
+  unsigned hist[kBins];   // this CTA's counts
+  unsigned total[kBins];  // in rank 0: the row's
+  unsigned warp_u[kSampleWarps];
+  unsigned count;  // in rank 0: tokens in the list
+  int mode, lo, hi, k_cut;
+  unsigned above, in;
+  int found, last;
+};
+
+enum SampleMode { kAll, kList, kWide, kBisect };
+
+// Floats as unsigned integers of the same order, and back.
 __device__ __forceinline__ uint32_t ordered_bits(float x) {
   const uint32_t b = __float_as_uint(x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-template <typename T>
-__device__ __forceinline__ T block_sum(T v, T* part) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) part[warp] = v;
-  __syncthreads();
-  v = part[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ u64 token_key(float l, int i) {
+  return (u64)ordered_bits(l) << 32 | (0xffffffffu - (uint32_t)i);
 }
 
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
-  __shared__ double part_d[32];
-  __shared__ int part_i[32];
-  __shared__ float part_f[32];
-  __shared__ int found;
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n = (int)a.vocab;
-  auto logit = [&](int i) {
-    const float l = ld_any(a.logits, r * a.row_stride + i, a.dtype);
-    return l != l ? -INFINITY : l;
-  };
-  float top = -INFINITY;
-  for (int i = tid; i < n; i += kSampleThreads) top = fmaxf(top, logit(i));
-  top = warp_max(top);
-  if (lane == 0) part_f[warp] = top;
-  if (tid == 0) found = n;
-  __syncthreads();
-  top = warp_max(part_f[lane]);
-  if (top == -INFINITY) {
-    if (tid == 0) a.ids[r] = -1;
-    return;
+// A logit as the definition takes it: NaN is -infinity, -0 is 0.
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.f; }
+
+// 2^t for -61 < t <= 0, 0 below.
+__device__ __forceinline__ double ex2_f64(double t, const double* tab) {
+  if (!(t > -61.0)) return 0.0;
+  const double round = 0x1.8p48;  // adding it leaves multiples of 1/16
+  const double z = t + round;
+  const int n = __double2loint(z);
+  const double r = t - (z - round);
+  double p = fma(0.00133335581464284434, r, 0.00961812910762847716);
+  p = fma(p, r, 0.05550410866482157995);
+  p = fma(p, r, 0.24022650695910071233);
+  p = fma(p, r, 0.69314718055994530942);
+  p = fma(p, r, 1.0) * tab[n & 15];
+  return __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p));
+}
+
+// f(value, index) for the row's tokens [a, b), a warp's run: lane by lane in
+// 16-byte words, each lane's indexes ascending.
+template <typename T, typename F>
+__device__ __forceinline__ void each_token(const T* row, int a, int b, F f) {
+  constexpr int VEC = 16 / (int)sizeof(T), U = sizeof(T) == 4 ? 4 : 2;
+  const int lane = threadIdx.x & 31;
+  const int mis = (int)((reinterpret_cast<uintptr_t>(row + a) / sizeof(T)) % VEC);
+  const int head = min(b - a, (VEC - mis) % VEC);
+  if (lane < head) f(clean(Elem<T>::to_f32(row[a + lane])), a + lane);
+  a += head;
+  const int words = (b - a) / VEC;
+  const uint4* src = reinterpret_cast<const uint4*>(row + a);
+  for (int v = lane; v < words; v += 32 * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (v + 32 * u < words) w[u] = src[v + 32 * u];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (v + 32 * u >= words) break;
+      const T* e = reinterpret_cast<const T*>(&w[u]);
+#pragma unroll
+      for (int k = 0; k < VEC; k++) f(clean(Elem<T>::to_f32(e[k])), a + (v + 32 * u) * VEC + k);
+    }
   }
+  a += words * VEC;
+  if (lane < b - a) f(clean(Elem<T>::to_f32(row[a + lane])), a + lane);
+}
+
+__device__ __forceinline__ double warp_sum_d(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// Exclusive running sum over the CTA's threads, and the total.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* part, V& all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  V run = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V t = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += t;
+  }
+  __syncthreads();
+  if (lane == 31) part[warp] = run;
+  __syncthreads();
+  V before = 0;
+  all = 0;
+  for (int w = 0; w < kSampleWarps; w++) {
+    if (w == warp) before = all;
+    all += part[w];
+  }
+  return before + run - v;
+}
+
+// Bitonic sort of n keys (a power of two), descending.
+__device__ __forceinline__ void sort_desc(u64* k, int n) {
+  for (int size = 2; size <= n; size *= 2)
+    for (int d = size / 2; d > 0; d /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kSampleThreads) {
+        const int x = 2 * i - (i & (d - 1)), y = x + d;
+        const u64 p = k[x], q = k[y];
+        if ((p < q) == ((x & size) == 0)) {
+          k[x] = q;
+          k[y] = p;
+        }
+      }
+    }
+  __syncthreads();
+}
+__device__ __forceinline__ int pow2_from(int n) {
+  int p = 2;
+  while (p < n) p *= 2;
+  return p;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SampleShared& s = *reinterpret_cast<SampleShared*>(smem_raw);
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = a.cluster, rank = blockIdx.x % C;
+  const int64_t r = blockIdx.x / C;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n = (int)a.vocab, runs = C * kSampleWarps;
+  const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
+  auto run_start = [&](int g) { return (int)((int64_t)n * g / runs); };
+  const int g = rank * kSampleWarps + warp, i0 = run_start(g), i1 = run_start(g + 1);
+  auto sync = [&]() {
+    if (C > 1) cl.sync();
+    else __syncthreads();
+  };
+  auto at_rank = [&](auto* p, int to) { return C > 1 ? cl.map_shared_rank(p, to) : p; };
+
   const float temp = a.temperature ? a.temperature[r] : 1.f;
-  if (!(temp > 0.f)) {
-    for (int i = tid; i < n; i += kSampleThreads)
-      if (logit(i) == top) atomicMin(&found, i);
+  const bool greedy = !(temp > 0.f);
+  const int top_k = a.top_k ? a.top_k[r] : 0;
+  const float top_p = a.top_p ? a.top_p[r] : 1.f;
+  const double min_p = a.min_p && a.min_p[r] > 0.f ? (double)a.min_p[r] : 0.0;
+  const bool k_on = !greedy && top_k > 0 && top_k < n, p_on = !greedy && top_p < 1.f;
+  // One variable decides which passes a row takes. (With the conditions
+  // spelled out at each branch nvcc 12.9 dropped the one before pass 2.)
+  enum Kind { kGreedy, kCut, kFloor, kOpen };
+  const int kind = greedy ? kGreedy : (k_on || p_on) ? kCut : min_p > 0.0 ? kFloor : kOpen;
+  const bool open = kind == kOpen;
+  float u = a.u[r];
+  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  const double c = 1.4426950408889634 / (double)temp;  // octaves per unit of logit
+
+  if (tid < 16) s.tab[tid] = exp2((double)tid / 16);
+  for (int i = tid; i < kBins; i += kSampleThreads) s.hist[i] = s.total[i] = 0;
+  if (tid == 0) {
+    s.count = 0;
+    s.found = n;
+    s.last = -1;
+  }
+  __syncthreads();
+
+  // ---- pass 1: the largest logit and where it comes first; open rows: the
+  // weights' sum too, against each thread's own largest so far
+  float top = -INFINITY;
+  int top_i = n;
+  double sum = 0;
+  if (open) {
+    each_token(row, i0, i1, [&](float l, int i) {
+      if (l > top) {
+        sum = top == -INFINITY ? 0.0 : sum * ex2_f64(((double)top - (double)l) * c, s.tab);
+        top = l;
+        top_i = i;
+        sum += 1.0;
+      } else if (l == top) {
+        sum += l == -INFINITY ? 0.0 : 1.0;
+      } else if (l > -INFINITY) {
+        sum += ex2_f64(((double)l - (double)top) * c, s.tab);
+      }
+    });
+  } else {
+    each_token(row, i0, i1, [&](float l, int i) {
+      if (l > top) {
+        top = l;
+        top_i = i;
+      }
+    });
+  }
+  {
+    u64 best = token_key(top, top_i);
+    const float mine = top;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const u64 t = __shfl_xor_sync(0xffffffffu, best, o);
+      best = t > best ? t : best;
+    }
+    top = from_ordered((uint32_t)(best >> 32));
+    if (open) {
+      // the run's sum against its largest
+      const double f = mine == top ? 1.0 : mine == -INFINITY ? 0.0 : ex2_f64(((double)mine - (double)top) * c, s.tab);
+      sum = warp_sum_d(top == -INFINITY ? 0.0 : sum * f);
+      if (lane < C) {
+        *at_rank(&s.seg[g], lane) = sum;
+        *at_rank(&s.seg_ref[g], lane) = top;
+      }
+    }
+    if (lane == 0) s.warp_best[warp] = best;
     __syncthreads();
-    if (tid == 0) a.ids[r] = found;
+    for (int w = 0; w < kSampleWarps; w++) best = s.warp_best[w] > best ? s.warp_best[w] : best;
+    if (tid < C) *at_rank(&s.best[rank], tid) = best;
+    sync();
+    for (int q = 0; q < C; q++) best = s.best[q] > best ? s.best[q] : best;
+    top = from_ordered((uint32_t)(best >> 32));
+    top_i = (int)(0xffffffffu - (uint32_t)best);
+  }
+  // From here on a CTA may leave where no other will read its memory again.
+  if (top == -INFINITY || kind == kGreedy) {
+    if (rank == 0 && tid == 0) a.ids[r] = top == -INFINITY ? -1 : top_i;
     return;
   }
   auto weight = [&](float l) {
     if (l == top) return 1.0;
     if (l == -INFINITY) return 0.0;
-    const double w = exp(((double)l - (double)top) / (double)temp);
+    const double w = ex2_f64(((double)l - (double)top) * c, s.tab);
     return w < 0x1p-60 ? 0.0 : w;
   };
-  auto key = [&](float l, int i) {
-    return (unsigned long long)ordered_bits(l) << 32 | (0xffffffffu - (uint32_t)i);
-  };
-  unsigned long long cut = 0;
-  auto mass = [&](unsigned long long at) {
-    double s = 0;
-    for (int i = tid; i < n; i += kSampleThreads) {
-      const float l = logit(i);
-      if (key(l, i) >= at) s += weight(l);
+
+  u64 cut = 0;
+  if (kind == kCut) {
+    // ---- pass 2: counts by bin; a token past the last bin has no weight
+    const float cb = (float)(c * kPerOctave);
+    auto bin_of = [&](float l) {
+      if (l == top) return 0;
+      float d = (top - l) * cb;  // not below 0, and not smaller for a smaller l
+      if (!(top - l <= 3.402823466e38f)) d = (float)(((double)top - (double)l) * (c * kPerOctave));
+      return d < (float)kBins ? (int)d : kBins;
+    };
+    each_token(row, i0, i1, [&](float l, int) {
+      const int b = bin_of(l);
+      if (b < kBins) atomicAdd(&s.hist[b], 1u);
+    });
+    __syncthreads();
+    if (C > 1) {
+      unsigned* to = cl.map_shared_rank(s.total, 0);
+      for (int i = tid; i < kBins; i += kSampleThreads)
+        if (s.hist[i]) atomicAdd(to + i, s.hist[i]);
     }
-    return block_sum(s, part_d);
-  };
-  const int k = a.top_k ? a.top_k[r] : 0;
-  if (k > 0 && k < n) {
-    for (int bit = 63; bit >= 0; bit--) {
-      const unsigned long long at = cut | 1ull << bit;
-      int c = 0;
-      for (int i = tid; i < n; i += kSampleThreads) c += key(logit(i), i) >= at;
-      if (block_sum(c, part_i) >= k) cut = at;
-    }
-  }
-  const float p = a.top_p ? a.top_p[r] : 1.f;
-  if (p < 1.f) {
-    const double want = (double)p * mass(cut);
-    const unsigned long long low = cut;
-    cut = 0;
-    for (int bit = 63; bit >= 0; bit--) {
-      const unsigned long long at = cut | 1ull << bit;
-      const double s = mass(at);
-      if (s >= want && s > 0) cut = at;
-    }
-    cut = cut > low ? cut : low;
-  }
-  const double least = a.min_p && a.min_p[r] > 0.f ? (double)a.min_p[r] : 0.0;
-  auto kept = [&](int i) {
-    const float l = logit(i);
-    if (key(l, i) < cut) return 0.0;
-    const double w = weight(l);
-    return w >= least || l == top ? w : 0.0;
-  };
-  // the running sum in the vocabulary's order: a run of tokens per thread
-  const int per = (n + kSampleThreads - 1) / kSampleThreads;
-  const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
-  double s = 0;
-  for (int i = i0; i < i1; i++) s += kept(i);
-  double run = s;
+    sync();
+    const unsigned* total = C > 1 ? s.total : s.hist;
+    if (rank == 0) {
+      // four bins to a thread: counts and estimated masses, from the top
+      constexpr int PER = 4;
+      unsigned cnt[PER], before, all;
+      double mass = 0, est[PER];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double t = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += t;
-  }
-  if (lane == 31) part_d[warp] = run;
-  __syncthreads();
-  double before = 0, total = 0;
-  for (int w = 0; w < 32; w++) {
-    if (w < warp) before += part_d[w];
-    total += part_d[w];
-  }
-  before += run - s;
-  float u = a.u[r];
-  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-  const double target = (double)u * total;
-  if (s > 0 && before + s > target) {
-    double c = before;
-    for (int i = i0; i < i1; i++) {
-      const double w = kept(i);
-      c += w;
-      if (w > 0 && c > target) {
-        atomicMin(&found, i);
-        break;
+      for (int j = 0; j < PER; j++) {
+        const int b = tid * PER + j;
+        cnt[j] = b < kBins ? total[b] : 0;
+        est[j] = cnt[j] * ex2_f64(-(b + 0.5) / kPerOctave, s.tab);
+        mass += est[j];
+      }
+      before = block_scan(cnt[0] + cnt[1] + cnt[2] + cnt[3], s.warp_u, all);
+      double m_all, m_before = block_scan(mass, s.warp_d, m_all);
+      const bool k_cut = k_on && (unsigned)top_k < all;  // else fewer tokens have weight
+      const double want = (double)fmaxf(top_p, 0x1p-100f) * m_all;
+      if (tid == 0) {
+        s.lo = 0;
+        s.hi = kBins - 1;  // where no bin is the cut's
+      }
+      __syncthreads();
+      unsigned run = before;
+      double m_run = m_before;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {  // the cut's bin
+        const bool here = k_cut ? run < (unsigned)top_k && run + cnt[j] >= (unsigned)top_k
+                                : m_run < want && m_run + est[j] >= want;
+        if (here && cnt[j]) atomicMin(&s.hi, tid * PER + j);
+        run += cnt[j];
+        m_run += est[j];
+      }
+      __syncthreads();
+      const int cut_bin = s.hi;
+      run = before;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        if (tid * PER + j == cut_bin) {
+          s.above = run;
+          s.in = cnt[j];
+        }
+        run += cnt[j];
+      }
+      __syncthreads();
+      const unsigned above = s.above, in = s.in;
+      int mode = kList;
+      if (!k_cut && !p_on) mode = kAll;
+      else if (in > kCap || (above + in > kCap && k_cut && p_on)) mode = kBisect;
+      else if (above + in > kCap) mode = kWide;
+      __syncthreads();
+      if (mode == kWide && tid == 0) s.lo = cut_bin;
+      __syncthreads();
+      // top_p's cut was estimated: take as many bins around as the list holds,
+      // below it first (half of the room left, in the wide case), then above
+      if (!k_cut && (mode == kList || mode == kWide)) {
+        const unsigned room = mode == kList ? kCap : above + in + (kCap - in) / 2;
+        run = before;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+          run += cnt[j];
+          const int b = tid * PER + j;
+          if (b > cut_bin && b < kBins && run <= room) atomicMax(&s.hi, b);
+        }
+        __syncthreads();
+        if (mode == kWide) {
+          const int hi = s.hi;
+          run = before;
+#pragma unroll
+          for (int j = 0; j < PER; j++) {
+            run += cnt[j];
+            if (tid * PER + j == hi) s.in = run;  // tokens down to hi
+          }
+          __syncthreads();
+          const unsigned down = s.in;
+          run = before;
+#pragma unroll
+          for (int j = 0; j < PER; j++) {
+            const int b = tid * PER + j;
+            if (b < cut_bin && down - run <= kCap) atomicMin(&s.lo, b);
+            run += cnt[j];
+          }
+          __syncthreads();
+        }
+      }
+      const int lo = s.lo, hi = s.hi;
+      if (tid < C) {
+        *at_rank(&s.mode, tid) = mode;
+        *at_rank(&s.lo, tid) = lo;
+        *at_rank(&s.hi, tid) = hi;
+        *at_rank(&s.k_cut, tid) = k_cut ? 1 : 0;
+      }
+    }
+    sync();
+    int mode = s.mode;
+    const int lo = s.lo, hi = s.hi;
+    const bool k_cut = s.k_cut != 0;
+
+    if (mode == kList || mode == kWide) {
+      // ---- pass 3: the window into rank 0's list; sums above it, and in all
+      double above = 0, whole = 0;
+      unsigned n_above = 0;
+      unsigned* counter = at_rank(&s.count, 0);
+      u64* list = at_rank(s.list, 0);
+      const bool sums = p_on && !k_cut, count = k_cut && lo > 0;
+      each_token(row, i0, i1, [&](float l, int i) {
+        const int b = bin_of(l);
+        if (b >= lo && b <= hi) {
+          const unsigned at = atomicAdd(counter, 1u);
+          if (at < kCap) list[at] = token_key(l, i);  // the window holds no more
+        }
+        if (sums) {
+          const double w = weight(l);
+          whole += w;
+          if (b < lo) above += w;
+        } else if (count && b < lo) {
+          n_above++;
+        }
+      });
+      if (sums || count) {
+        double all_a, all_w = 0;
+        if (count) above = n_above;
+        block_scan(above, s.warp_d, all_a);
+        if (sums) block_scan(whole, s.warp_d, all_w);
+        if (tid == 0) {
+          *at_rank(&s.part[0][0][rank], 0) = all_a;
+          *at_rank(&s.part[0][1][rank], 0) = all_w;
+        }
+      }
+      sync();
+      if (rank == 0) {
+        const int m = min((int)s.count, kCap), size = pow2_from(m);
+        for (int i = m + tid; i < size; i += kSampleThreads) s.list[i] = 0;
+        sort_desc(s.list, size);
+        above = whole = 0;
+        if (sums || count)
+          for (int q = 0; q < C; q++) {
+            above += s.part[0][0][q];
+            whole += s.part[0][1][q];
+          }
+        // running sums of the sorted list's weights, four to a thread
+        constexpr int PER = kCap / kSampleThreads;
+        double w[PER], mine = 0, all, b4[PER];
+        const int left = k_cut ? top_k - (count ? (int)above : 0) : m;  // places in the list
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+          const int i = tid * PER + j;
+          w[j] = i < m && i < left ? weight(from_ordered((uint32_t)(s.list[i] >> 32))) : 0.0;
+          b4[j] = mine;
+          mine += w[j];
+        }
+        const double start = block_scan(mine, s.warp_d, all) + (sums ? above : 0.0);
+        if (!sums) whole = all;  // of the top_k tokens, or of all that have weight
+        const double want = (double)top_p * whole;
+        unsigned keep = 0, kept;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+          const int i = tid * PER + j;
+          const bool first = i == 0 && lo == 0;
+          if (i < m && i < left && (first || !p_on || count || start + b4[j] < want) &&
+              (first || w[j] >= min_p))
+            keep++;
+        }
+        block_scan(keep, s.warp_u, kept);
+        // top_p's cut is not in the window: above it, or below
+        const bool missed = sums && ((lo > 0 && above >= want) ||
+                                     ((int)kept == m && hi + 1 < kBins && above + all < want));
+        if (missed) mode = kBisect;
+        if (mode == kList) {
+          // all kept tokens are here: in index order, the running sum again
+          const int size2 = pow2_from((int)kept);
+          u64 k2[PER];
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < PER; j++) k2[j] = tid * PER + j < (int)kept ? s.list[tid * PER + j] : 0;
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < PER; j++)  // complemented index first: descending is index ascending
+            if (tid * PER + j < size2) s.list[tid * PER + j] = k2[j] << 32 | k2[j] >> 32;
+          sort_desc(s.list, size2);
+          mine = 0;
+#pragma unroll
+          for (int j = 0; j < PER; j++) {
+            const int i = tid * PER + j;
+            w[j] = i < (int)kept ? weight(from_ordered((uint32_t)s.list[i])) : 0.0;
+            mine += w[j];
+          }
+          double run = block_scan(mine, s.warp_d, all);
+          const double target = (double)u * all;
+          // the first place at which the sum passes the target
+#pragma unroll
+          for (int j = 0; j < PER; j++) {
+            const int i = tid * PER + j;
+            run += w[j];
+            if (w[j] > 0) {
+              if (run > target) atomicMin(&s.found, i);
+              atomicMax(&s.last, i);
+            }
+          }
+          __syncthreads();
+          if (tid == 0) {
+            const int i = s.found < n ? s.found : s.last;
+            a.ids[r] = (int)(0xffffffffu - (uint32_t)(s.list[i] >> 32));
+          }
+        } else if (mode == kWide) {
+          // the last kept key; none in the window: what is above its first
+          if (tid == 0) s.cut = kept > 0 ? s.list[kept - 1] : s.list[0] + 1;
+          __syncthreads();
+        }
+        if (tid < C) {
+          *at_rank(&s.mode, tid) = mode;
+          *at_rank(&s.cut, tid) = s.cut;
+        }
+      }
+      if (mode == kList) {
+        // rank 0 alone knows whether the list sufficed
+        sync();
+        if (s.mode == kList) return;
+      } else {
+        sync();
+      }
+      mode = s.mode;
+      cut = s.cut;
+    }
+    if (mode == kBisect) {
+      // ---- a pass per bit of the key: counts, then exact sums
+      int turn = 0;
+      auto reduce = [&](double v) {
+        double all;
+        block_scan(v, s.warp_d, all);
+        if (tid < C) *at_rank(&s.part[turn & 1][0][rank], tid) = all;
+        sync();
+        all = 0;
+        for (int q = 0; q < C; q++) all += s.part[turn & 1][0][q];
+        turn++;
+        return all;
+      };
+      cut = 0;
+      if (k_on)
+        for (int bit = 63; bit >= 0; bit--) {
+          const u64 at = cut | 1ull << bit;
+          int v = 0;
+          each_token(row, i0, i1, [&](float l, int i) { v += token_key(l, i) >= at; });
+          if (reduce(v) >= top_k) cut = at;
+        }
+      if (p_on) {
+        const u64 low = cut;
+        auto mass = [&](u64 at) {
+          double v = 0;
+          each_token(row, i0, i1, [&](float l, int i) {
+            if (token_key(l, i) >= at) v += weight(l);
+          });
+          return reduce(v);
+        };
+        const double want = (double)top_p * mass(low);
+        cut = 0;
+        for (int bit = 63; bit >= 0; bit--) {
+          const u64 at = cut | 1ull << bit;
+          const double v = mass(at);
+          if (v >= want && v > 0) cut = at;
+        }
+        cut = cut > low ? cut : low;
       }
     }
   }
-  __syncthreads();
-  if (tid == 0) a.ids[r] = found;
-}
 
-cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
-  sample_kernel<<<(unsigned)a.rows, kSampleThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  // ---- pass 4: sums of the kept weights by run; open rows have them
+  auto kept_weight = [&](float l, int i) {
+    if (token_key(l, i) < cut) return 0.0;
+    const double w = weight(l);
+    return w >= min_p || l == top ? w : 0.0;
+  };
+  double before = 0, total = 0;
+  if (open) {
+    for (int q = 0; q < runs; q++) {
+      const float ref = s.seg_ref[q];
+      total += s.seg[q] * weight(ref);
+    }
+  } else {
+    sum = 0;
+    each_token(row, i0, i1, [&](float l, int i) { sum += kept_weight(l, i); });
+    sum = warp_sum_d(sum);
+    if (lane < C) *at_rank(&s.seg[g], lane) = sum;
+    sync();
+    for (int q = 0; q < runs; q++) total += s.seg[q];
+  }
+  const double target = (double)u * total;
+  int run = -1;
+  {
+    double at = 0;
+    for (int q = 0; q < runs; q++) {
+      const double v = open ? s.seg[q] * weight(s.seg_ref[q]) : s.seg[q];
+      if (v > 0) {
+        run = q;
+        before = at;
+        if (at + v > target) break;
+      }
+      at += v;
+    }
+  }
+  if (run / kSampleWarps != rank) return;
+
+  // ---- the run, in pieces of consecutive tokens to a thread
+  const int a0 = run_start(run), a1 = run_start(run + 1);
+  const int per = (a1 - a0 + kSampleThreads - 1) / kSampleThreads;
+  const int b0 = min(a1, a0 + tid * per), b1 = min(a1, b0 + per);
+  sum = 0;
+  for (int i = b0; i < b1; i++) sum += kept_weight(clean(Elem<T>::to_f32(row[i])), i);
+  double all;
+  double at = before + block_scan(sum, s.warp_d, all);
+  for (int i = b0; i < b1 && sum > 0; i++) {
+    const double w = kept_weight(clean(Elem<T>::to_f32(row[i])), i);
+    at += w;
+    if (w > 0) {
+      if (at > target) {
+        atomicMin(&s.found, i);
+        break;
+      }
+      atomicMax(&s.last, i);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) a.ids[r] = s.found < n ? s.found : s.last;
 }
 
 size_t sample_workspace_bytes(int64_t, int64_t) { return 0; }
+
+template <typename T>
+static cudaError_t run_sample(SampleArgs a, cudaStream_t st) {
+  auto kern = sample_kernel<T>;
+  static unsigned configured = 0;
+  const cudaError_t e = allow_smem(kern, (int)sizeof(SampleShared), &configured);
+  if (e != cudaSuccess) return e;
+  // Two CTAs for every SM while rows are few, each with 4096 tokens at least.
+  a.cluster = 1;
+  while (a.cluster < kMaxCluster && a.rows * a.cluster * 2 <= 2 * sm_count() &&
+         a.vocab >= 4096 * 2 * a.cluster)
+    a.cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.rows * a.cluster));
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = sizeof(SampleShared);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
+  switch (a.dtype) {
+    case kF32: return run_sample<float>(a, st);
+    case kF16: return run_sample<__half>(a, st);
+    default: return run_sample<__nv_bfloat16>(a, st);
+  }
+}
 
 }  // namespace eb

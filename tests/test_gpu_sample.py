@@ -119,6 +119,18 @@ def test_odd_uniforms(eb, u):
     _check(eb, _logits(12, 3333, 6, spread=40.0), u)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 40, 100, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.97, temperature=1.3),
+                                dict(top_k=5000, temperature=2.0), dict(top_k=3000, top_p=0.95),
+                                dict(min_p=0.001, temperature=1.5), dict(top_p=0.99, min_p=0.0001)])
+def test_row_counts_and_wide_cuts(eb, rows, dtype, kw):
+    """Few rows share a cluster of CTAs, many have one each; cuts behind some tokens and behind tens of
+    thousands."""
+    rng = np.random.default_rng(rows)
+    _check(eb, _logits(rows, 60013, rows, dtype, 2.0), rng.random(rows).astype(np.float32), **kw)
+
+
 def test_rows_with_settings_of_their_own(eb):
     rng = np.random.default_rng(0)
     rows = 60
