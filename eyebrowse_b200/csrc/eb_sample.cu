@@ -22,8 +22,8 @@
 //           which u's share falls is then walked by its CTA. With all kept
 //           tokens in the list, the list sorted by index takes its place.
 //
-// Weights are f64 (2^t by a 16-entry table and a Taylor polynomial of degree
-// 5: 2 * 10^-13 relative): in f32 the running sum over a vocabulary would be
+// Weights are f64 (2^t by a 32-entry table and a Taylor polynomial of degree
+// 4: 2 * 10^-12 relative): in f32 the running sum over a vocabulary would be
 // off by more than many a token's share. Sums meet in a fixed order, so
 // results do not depend on timing (the list's order of arrival is undone by
 // the sort).
@@ -51,7 +51,7 @@ typedef unsigned long long u64;
 
 struct SampleShared {
   u64 list[kCap];
-  double tab[16];
+  double tab[32];
   double seg[kMaxCluster * kSampleWarps];  // sums of the row's runs
   float seg_ref[kMaxCluster * kSampleWarps];
   double part[2][2][kMaxCluster];  // CTAs' sums, by turn
@@ -85,33 +85,45 @@ __device__ __forceinline__ u64 token_key(float l, int i) {
 // A logit as the definition takes it: NaN is -infinity, -0 is 0.
 __device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.f; }
 
-// 2^t for -61 < t <= 0, 0 below.
-__device__ __forceinline__ double ex2_f64(double t, const double* tab) {
-  if (!(t > -61.0)) return 0.0;
-  const double round = 0x1.8p48;  // adding it leaves multiples of 1/16
-  const double z = t + round;
+// Taylor coefficients of 2^r and the rounding constant, as operands of the
+// f64 instructions (an immediate would take two moves).
+__constant__ double kEx2[5] = {0.69314718055994530942, 0.24022650695910071233,
+                               0.05550410866482157995, 0.00961812910762847716, 0x1.8p47};
+
+// 2^t for -61 < t <= 0 (1 exactly for 0); elsewhere and for NaN see `on`.
+__device__ __forceinline__ double ex2_raw(double t, const double* tab) {
+  const double z = t + kEx2[4];  // multiples of 1/32 in its lowest bits
   const int n = __double2loint(z);
-  const double r = t - (z - round);
-  double p = fma(0.00133335581464284434, r, 0.00961812910762847716);
-  p = fma(p, r, 0.05550410866482157995);
-  p = fma(p, r, 0.24022650695910071233);
-  p = fma(p, r, 0.69314718055994530942);
-  p = fma(p, r, 1.0) * tab[n & 15];
-  return __hiloint2double(__double2hiint(p) + (n >> 4) * (1 << 20), __double2loint(p));
+  const double r = t - (z - kEx2[4]);  // |r| <= 1/64
+  const double q = fma(fma(fma(kEx2[3], r, kEx2[2]), r, kEx2[1]), r, kEx2[0]);
+  const double v = tab[n & 31];
+  const double p = fma(v * r, q, v);
+  return __hiloint2double((int)((unsigned)__double2hiint(p) + ((unsigned)(n >> 5) << 20)),
+                          __double2loint(p));
+}
+__device__ __forceinline__ double ex2_f64(double t, const double* tab) {
+  return t > -61.0 ? ex2_raw(t, tab) : 0.0;
 }
 
-// f(value, index) for the row's tokens [a, b), a warp's run: lane by lane in
-// 16-byte words, each lane's indexes ascending.
+// f(values, first index) for the row's tokens [a, b), a warp's run, in 16-byte
+// words, each lane's indexes ascending. At the ends single tokens come, padded
+// with -infinity.
 template <typename T, typename F>
-__device__ __forceinline__ void each_token(const T* row, int a, int b, F f) {
+__device__ __forceinline__ void each_word(const T* row, int a, int b, F f) {
   constexpr int VEC = 16 / (int)sizeof(T), U = sizeof(T) == 4 ? 4 : 2;
   const int lane = threadIdx.x & 31;
   const int mis = (int)((reinterpret_cast<uintptr_t>(row + a) / sizeof(T)) % VEC);
   const int head = min(b - a, (VEC - mis) % VEC);
-  if (lane < head) f(clean(Elem<T>::to_f32(row[a + lane])), a + lane);
-  a += head;
-  const int words = (b - a) / VEC;
-  const uint4* src = reinterpret_cast<const uint4*>(row + a);
+  const int words = (b - a - head) / VEC, tail = b - a - head - words * VEC;
+  float l[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; k++) l[k] = -INFINITY;
+  if (lane < head) {
+    l[0] = clean(Elem<T>::to_f32(row[a + lane]));
+    f(l, a + lane);
+  }
+  const int a1 = a + head;
+  const uint4* src = reinterpret_cast<const uint4*>(row + a1);
   for (int v = lane; v < words; v += 32 * U) {
     uint4 w[U];
 #pragma unroll
@@ -119,14 +131,29 @@ __device__ __forceinline__ void each_token(const T* row, int a, int b, F f) {
       if (v + 32 * u < words) w[u] = src[v + 32 * u];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (v + 32 * u >= words) break;
-      const T* e = reinterpret_cast<const T*>(&w[u]);
+      if (v + 32 * u < words) {
+        const T* e = reinterpret_cast<const T*>(&w[u]);
+        float x[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; k++) f(clean(Elem<T>::to_f32(e[k])), a + (v + 32 * u) * VEC + k);
+        for (int k = 0; k < VEC; k++) x[k] = clean(Elem<T>::to_f32(e[k]));
+        f(x, a1 + (v + 32 * u) * VEC);
+      }
     }
   }
-  a += words * VEC;
-  if (lane < b - a) f(clean(Elem<T>::to_f32(row[a + lane])), a + lane);
+  if (lane < tail) {
+    l[0] = clean(Elem<T>::to_f32(row[b - tail + lane]));
+    f(l, b - tail + lane);
+  }
+}
+// f(value, index). What each_word pads its words with comes too: -infinity,
+// which has no weight, no bin and no place among the largest.
+template <typename T, typename F>
+__device__ __forceinline__ void each_token(const T* row, int a, int b, F f) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  each_word<T>(row, a, b, [&](const float (&l)[VEC], int i) {
+#pragma unroll
+    for (int k = 0; k < VEC; k++) f(l[k], i + k);
+  });
 }
 
 __device__ __forceinline__ double warp_sum_d(double x) {
@@ -212,7 +239,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
   u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
   const double c = 1.4426950408889634 / (double)temp;  // octaves per unit of logit
 
-  if (tid < 16) s.tab[tid] = exp2((double)tid / 16);
+  if (tid < 32) s.tab[tid] = exp2((double)tid / 32);
   for (int i = tid; i < kBins; i += kSampleThreads) s.hist[i] = s.total[i] = 0;
   if (tid == 0) {
     s.count = 0;
@@ -227,16 +254,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
   int top_i = n;
   double sum = 0;
   if (open) {
-    each_token(row, i0, i1, [&](float l, int i) {
-      if (l > top) {
-        sum = top == -INFINITY ? 0.0 : sum * ex2_f64(((double)top - (double)l) * c, s.tab);
-        top = l;
-        top_i = i;
-        sum += 1.0;
-      } else if (l == top) {
-        sum += l == -INFINITY ? 0.0 : 1.0;
-      } else if (l > -INFINITY) {
-        sum += ex2_f64(((double)l - (double)top) * c, s.tab);
+    constexpr int VEC = 16 / (int)sizeof(T);
+    double far = 0;  // the thread's largest
+    each_word<T>(row, i0, i1, [&](const float (&l)[VEC], int i) {
+      float m = l[0];
+#pragma unroll
+      for (int k = 1; k < VEC; k++) m = fmaxf(m, l[k]);
+      if (m > top) {
+        sum = top == -INFINITY ? 0.0 : sum * ex2_f64(((double)top - (double)m) * c, s.tab);
+        top = m;
+        far = (double)m;
+      }
+      if (top == INFINITY) {
+#pragma unroll
+        for (int k = 0; k < VEC; k++) sum += l[k] == INFINITY ? 1.0 : 0.0;
+      } else if (top > -INFINITY) {
+        // -infinity leaves t -infinity or NaN: not counted
+#pragma unroll
+        for (int k = 0; k < VEC; k++) {
+          const double t = ((double)l[k] - far) * c;  // 0 for the largest itself
+          const double w = ex2_raw(t, s.tab);
+          if (t > -61.0) sum += w;
+        }
       }
     });
   } else {
@@ -279,27 +318,45 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
     if (rank == 0 && tid == 0) a.ids[r] = top == -INFINITY ? -1 : top_i;
     return;
   }
-  auto weight = [&](float l) {
-    if (l == top) return 1.0;
-    if (l == -INFINITY) return 0.0;
-    const double w = ex2_f64(((double)l - (double)top) * c, s.tab);
-    return w < 0x1p-60 ? 0.0 : w;
+  const double top_d = (double)top;
+  auto weight = [&](float l) {  // -infinity leaves t -infinity or NaN: none
+    const double t = ((double)l - top_d) * c;
+    const double w = ex2_raw(t, s.tab);
+    return l == top ? 1.0 : t >= -60.0 ? w : 0.0;
+  };
+
+  // 1/32 octaves of weight below the largest; a token past the last bin has none.
+  const float cb = (float)(c * kPerOctave);
+  auto bin_of = [&](float l) {
+    if (l == top) return 0;
+    float d = (top - l) * cb;  // not below 0, and not smaller for a smaller l
+    if (!(top - l <= 3.402823466e38f)) d = (float)(((double)top - (double)l) * (c * kPerOctave));
+    return d < (float)kBins ? (int)d : kBins;
   };
 
   u64 cut = 0;
+  double above = 0;          // this thread's tokens above the window
+  int win_lo = 0, win_hi = -1;  // and the window: pass 4 reads it alone
   if (kind == kCut) {
-    // ---- pass 2: counts by bin; a token past the last bin has no weight
-    const float cb = (float)(c * kPerOctave);
-    auto bin_of = [&](float l) {
-      if (l == top) return 0;
-      float d = (top - l) * cb;  // not below 0, and not smaller for a smaller l
-      if (!(top - l <= 3.402823466e38f)) d = (float)(((double)top - (double)l) * (c * kPerOctave));
-      return d < (float)kBins ? (int)d : kBins;
-    };
-    each_token(row, i0, i1, [&](float l, int) {
-      const int b = bin_of(l);
-      if (b < kBins) atomicAdd(&s.hist[b], 1u);
-    });
+    // ---- pass 2: counts by bin
+    // for top_p alone, the sum of all weights too
+    const bool sums = p_on && !k_on;
+    double whole = 0;
+    if (sums) {
+      each_token(row, i0, i1, [&](float l, int) {
+        const int b = bin_of(l);
+        if (b < kBins) atomicAdd(&s.hist[b], 1u);
+        whole += weight(l);
+      });
+      double all;
+      block_scan(whole, s.warp_d, all);
+      if (tid == 0) *at_rank(&s.part[0][1][rank], 0) = all;
+    } else {
+      each_token(row, i0, i1, [&](float l, int) {
+        const int b = bin_of(l);
+        if (b < kBins) atomicAdd(&s.hist[b], 1u);
+      });
+    }
     __syncthreads();
     if (C > 1) {
       unsigned* to = cl.map_shared_rank(s.total, 0);
@@ -354,7 +411,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       const unsigned above = s.above, in = s.in;
       int mode = kList;
       if (!k_cut && !p_on) mode = kAll;
-      else if (in > kCap || (above + in > kCap && k_cut && p_on)) mode = kBisect;
+      else if (in > kCap || (k_on && p_on && (k_cut ? above + in : all) > kCap)) mode = kBisect;
       else if (above + in > kCap) mode = kWide;
       __syncthreads();
       if (mode == kWide && tid == 0) s.lo = cut_bin;
@@ -405,51 +462,48 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
     const bool k_cut = s.k_cut != 0;
 
     if (mode == kList || mode == kWide) {
-      // ---- pass 3: the window into rank 0's list; sums above it, and in all
-      double above = 0, whole = 0;
+      // ---- pass 3: the window into rank 0's list, the sum (for top_k: the
+      // count) of what is above it
       unsigned n_above = 0;
       unsigned* counter = at_rank(&s.count, 0);
       u64* list = at_rank(s.list, 0);
-      const bool sums = p_on && !k_cut, count = k_cut && lo > 0;
-      each_token(row, i0, i1, [&](float l, int i) {
-        const int b = bin_of(l);
+      const bool count = k_cut && lo > 0;
+      auto gather = [&](float l, int i, int b) {
         if (b >= lo && b <= hi) {
           const unsigned at = atomicAdd(counter, 1u);
           if (at < kCap) list[at] = token_key(l, i);  // the window holds no more
         }
-        if (sums) {
-          const double w = weight(l);
-          whole += w;
-          if (b < lo) above += w;
-        } else if (count && b < lo) {
-          n_above++;
-        }
-      });
-      if (sums || count) {
-        double all_a, all_w = 0;
-        if (count) above = n_above;
-        block_scan(above, s.warp_d, all_a);
-        if (sums) block_scan(whole, s.warp_d, all_w);
-        if (tid == 0) {
-          *at_rank(&s.part[0][0][rank], 0) = all_a;
-          *at_rank(&s.part[0][1][rank], 0) = all_w;
-        }
+      };
+      if (lo == 0) {
+        each_token(row, i0, i1, [&](float l, int i) { gather(l, i, bin_of(l)); });
+      } else {
+        each_token(row, i0, i1, [&](float l, int i) {
+          const int b = bin_of(l);
+          gather(l, i, b);
+          if (b < lo) {
+            above += weight(l);
+            n_above++;
+          }
+        });
+        double all_a;
+        block_scan(count ? (double)n_above : above, s.warp_d, all_a);
+        if (tid == 0) *at_rank(&s.part[0][0][rank], 0) = all_a;
       }
       sync();
       if (rank == 0) {
         const int m = min((int)s.count, kCap), size = pow2_from(m);
         for (int i = m + tid; i < size; i += kSampleThreads) s.list[i] = 0;
         sort_desc(s.list, size);
-        above = whole = 0;
-        if (sums || count)
-          for (int q = 0; q < C; q++) {
-            above += s.part[0][0][q];
-            whole += s.part[0][1][q];
-          }
+        double over = 0;  // of what is above the window
+        whole = 0;
+        for (int q = 0; q < C; q++) {
+          if (lo > 0) over += s.part[0][0][q];
+          if (sums) whole += s.part[0][1][q];
+        }
         // running sums of the sorted list's weights, four to a thread
         constexpr int PER = kCap / kSampleThreads;
         double w[PER], mine = 0, all, b4[PER];
-        const int left = k_cut ? top_k - (count ? (int)above : 0) : m;  // places in the list
+        const int left = k_cut ? top_k - (count ? (int)over : 0) : m;  // places in the list
 #pragma unroll
         for (int j = 0; j < PER; j++) {
           const int i = tid * PER + j;
@@ -457,7 +511,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
           b4[j] = mine;
           mine += w[j];
         }
-        const double start = block_scan(mine, s.warp_d, all) + (sums ? above : 0.0);
+        const double start = block_scan(mine, s.warp_d, all) + (sums ? over : 0.0);
         if (!sums) whole = all;  // of the top_k tokens, or of all that have weight
         const double want = (double)top_p * whole;
         unsigned keep = 0, kept;
@@ -471,8 +525,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
         }
         block_scan(keep, s.warp_u, kept);
         // top_p's cut is not in the window: above it, or below
-        const bool missed = sums && ((lo > 0 && above >= want) ||
-                                     ((int)kept == m && hi + 1 < kBins && above + all < want));
+        const bool missed = sums && ((lo > 0 && over >= want) ||
+                                     ((int)kept == m && hi + 1 < kBins && over + all < want));
         if (missed) mode = kBisect;
         if (mode == kList) {
           // all kept tokens are here: in index order, the running sum again
@@ -529,6 +583,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       }
       mode = s.mode;
       cut = s.cut;
+      if (mode == kWide && min_p == 0.0) {
+        win_lo = lo;
+        win_hi = hi;
+      }
     }
     if (mode == kBisect) {
       // ---- a pass per bit of the key: counts, then exact sums
@@ -585,8 +643,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       total += s.seg[q] * weight(ref);
     }
   } else {
-    sum = 0;
-    each_token(row, i0, i1, [&](float l, int i) { sum += kept_weight(l, i); });
+    if (win_hi >= 0) {
+      sum = above;
+      each_token(row, i0, i1, [&](float l, int i) {
+        const int b = bin_of(l);
+        if (b >= win_lo && b <= win_hi) sum += kept_weight(l, i);
+      });
+    } else {
+      sum = 0;
+      each_token(row, i0, i1, [&](float l, int i) { sum += kept_weight(l, i); });
+    }
     sum = warp_sum_d(sum);
     if (lane < C) *at_rank(&s.seg[g], lane) = sum;
     sync();
@@ -606,7 +672,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
       at += v;
     }
   }
-  if (run / kSampleWarps != rank) return;
+  if (run < 0 || run / kSampleWarps != rank) return;  // (the largest has weight: some run has)
 
   // ---- the run, in pieces of consecutive tokens to a thread
   const int a0 = run_start(run), a1 = run_start(run + 1);
