@@ -26,6 +26,13 @@ the RMSNorms through eb_rmsnorm. The embedding gather, residual adds, the
 gated activations, the residual scalar and the softcap are torch
 element-wise operations. Sliding-window layers get their window in the
 descriptor (HF's semantics; the reference itself does not window yet).
+
+A decode step with fewer bytes (no reference counterpart): w4_group keeps the
+layers' projections in 4 bits with a scale per group (eb_w4_quantize,
+eb_linear_w4), cache="e4m3" or "e5m2" the K/V rows in 8 bits (prompts attend
+their own rows as they are, in an f32 cache that the layers share, and
+eb_kv8_write then stores them; eb_attention_decode_kv8 decodes), and generate
+draws tokens with eb_sample when it is given uniform numbers.
 """
 from __future__ import annotations
 
@@ -75,9 +82,13 @@ def spec_from_config(cfg: dict) -> dict:
 
 class DecoderModel:
     """A decoder on one GPU. `weights`: {HF tensor name: numpy array} (linear
-    and embedding weights f16-valued, as the reference stores them)."""
+    and embedding weights f16-valued, as the reference stores them).
+    w4_group: 32, 64 or 128 for 4-bit projections (w4_zero_point: with zero
+    points), 0 for f16. cache: "f32", "e4m3" or "e5m2"; kv_block: cache rows
+    per scale of the 8-bit types."""
 
-    def __init__(self, weights: dict, config: dict, max_seq: int):
+    def __init__(self, weights: dict, config: dict, max_seq: int, w4_group: int = 0,
+                 w4_zero_point: bool = False, cache: str = "f32", kv_block: int = 64):
         import torch
 
         import eyebrowse_b200 as eb
@@ -87,6 +98,18 @@ class DecoderModel:
         f16 = lambda *names: torch.from_numpy(np.ascontiguousarray(
             np.concatenate([weights[n] for n in names]).astype(np.float16))).cuda()
         H, Hkv, D, inter = s["heads"], s["kv_heads"], s["hidden"], s["inter"]
+        if cache not in ("f32", "e4m3", "e5m2"):
+            raise ValueError(f"cache {cache!r}: f32, e4m3 or e5m2")
+        self.kv8 = {"e4m3": eb.EB_E4M3, "e5m2": eb.EB_E5M2}.get(cache)
+        self.shared = {}  # head_dim -> the f32 cache that prompts of every layer pass through
+
+        def lin(*names):
+            if not w4_group:
+                return f16(*names)
+            w = np.concatenate([weights[n] for n in names]).astype(np.float32)
+            parts = eb.w4_quantize(w, w4_group, w4_zero_point)
+            return eb.make_w4(*(None if a is None else torch.from_numpy(a).cuda() for a in parts),
+                              w.shape[1], w.shape[0], w4_group)
         self.vec = {k: dev(v) for k, v in weights.items()
                     if k.endswith("norm.weight") or k.endswith("layer_scalar")}
         self.embed = dev(weights["model.embed_tokens.weight"])
@@ -105,20 +128,38 @@ class DecoderModel:
             qn = self.vec[f"{p}.self_attn.q_norm.weight"] if ly["qk_norm"] else None
             kn = self.vec[f"{p}.self_attn.k_norm.weight"] if ly["qk_norm"] else None
             shape = (max_seq, Hkv, hd)
-            self.L.append(dict(
+            ly_dev = dict(
                 hd=hd, width=width, desc=desc, layer=eb.make_layer(qn, kn, vw, cos, sin),
                 keep=(cos, sin, vw),
-                qkv=f16(f"{p}.self_attn.q_proj.weight", f"{p}.self_attn.k_proj.weight",
+                qkv=lin(f"{p}.self_attn.q_proj.weight", f"{p}.self_attn.k_proj.weight",
                         f"{p}.self_attn.v_proj.weight"),
-                o=f16(f"{p}.self_attn.o_proj.weight"),
-                gate_up=f16(f"{p}.mlp.gate_proj.weight", f"{p}.mlp.up_proj.weight"),
-                down=f16(f"{p}.mlp.down_proj.weight"),
-                kc=torch.zeros(shape, device="cuda"), vc=torch.zeros(shape, device="cuda"),
+                o=lin(f"{p}.self_attn.o_proj.weight"),
+                gate_up=lin(f"{p}.mlp.gate_proj.weight", f"{p}.mlp.up_proj.weight"),
+                down=lin(f"{p}.mlp.down_proj.weight"),
                 ws_prefill=eb.alloc_workspace(eb.attention_prefill_workspace_bytes(desc,
-                                                                                   max_seq)),
-                ws_decode=eb.alloc_workspace(eb.attention_decode_workspace_bytes(
-                    desc, 1, max_seq - 1))))
-            nb_lin = max([nb_lin] + [eb.linear_f16w_workspace_bytes(max_seq, k, n) for k, n in
+                                                                                   max_seq)))
+            if self.kv8 is None:
+                ly_dev.update(kc=torch.zeros(shape, device="cuda"),
+                              vc=torch.zeros(shape, device="cuda"),
+                              ws_decode=eb.alloc_workspace(eb.attention_decode_workspace_bytes(
+                                  desc, 1, max_seq - 1)))
+            else:
+                if hd not in self.shared:
+                    self.shared[hd] = tuple(torch.zeros(shape, device="cuda") for _ in range(2))
+                kc, vc = (torch.zeros(shape, dtype=torch.uint8, device="cuda") for _ in range(2))
+                blocks = (-(-max_seq // kv_block), Hkv)
+                ks, vs = (torch.zeros(blocks, device="cuda") for _ in range(2))
+                # the projections' fused rows, and the shared cache's own
+                d8, rows8 = (eb.make_desc(H, Hkv, hd, max_seq, dtype_cache=self.kv8, eps=s["eps"],
+                                          scale=ly["scale"], q_stride=w, kv_stride=w,
+                                          window=ly["window"]) for w in (width, 0))
+                ly_dev.update(kc=kc, vc=vc, kv8=eb.make_kv8(kc, vc, ks, vs, kv_block), desc8=d8,
+                              rows8=rows8,
+                              ws_decode=eb.alloc_workspace(eb.attention_decode_kv8_workspace_bytes(
+                                  d8, 1, max_seq - 1)))
+            self.L.append(ly_dev)
+            need = eb.linear_w4_workspace_bytes if w4_group else eb.linear_f16w_workspace_bytes
+            nb_lin = max([nb_lin] + [need(max_seq, k, n) for k, n in
                                      ((D, width), (H * hd, D), (D, 2 * inter), (inter, D))])
         self.ws_linear = eb.alloc_workspace(nb_lin) if nb_lin else None
 
@@ -135,8 +176,12 @@ class DecoderModel:
 
     def _linear(self, x, w):
         import torch
-        x = x.contiguous()
         rows, in_f = x.shape
+        if isinstance(w, self.eb.W4):
+            y = torch.empty(rows, w.out_f, device="cuda")
+            self.eb.linear_w4(w, x, y, rows, self.ws_linear)
+            return y
+        x = x.contiguous()
         y = torch.empty(rows, w.shape[0], device="cuda")
         self.eb.linear_f16w(x, w, y, rows, in_f, w.shape[0], self.ws_linear)
         return y
@@ -150,7 +195,15 @@ class DecoderModel:
         qkv = self._linear(h[:rows], ly["qkv"])
         q, k, v = qkv[:, :H * hd], qkv[:, H * hd:(H + Hkv) * hd], qkv[:, (H + Hkv) * hd:]
         o = torch.empty(rows, H * hd, device="cuda")
-        if prefill:
+        if prefill and self.kv8 is not None:
+            kc, vc = self.shared[hd]
+            eb.attention_prefill(ly["desc"], ly["layer"], rows, q, k, v, kc, vc, o,
+                                 ly["ws_prefill"])
+            eb.kv8_write(ly["rows8"], None, ly["kv8"], 0, rows, kc, vc)
+        elif self.kv8 is not None:
+            eb.attention_decode_kv8(ly["desc8"], ly["layer"], ly["kv8"], 1, None, base_pos, q, k, v,
+                                    o, ly["ws_decode"])
+        elif prefill:
             eb.attention_prefill(ly["desc"], ly["layer"], rows, q, k, v, ly["kc"], ly["vc"], o,
                                  ly["ws_prefill"])
         else:
@@ -197,15 +250,32 @@ class DecoderModel:
             out = cap * torch.tanh(out / cap)
         return out
 
-    def generate(self, prompt, n_new: int) -> list:
-        """Greedy ids: prefill the prompt, then decode one token at a time."""
+    def generate(self, prompt, n_new: int, uniforms=None, temperature: float = 1.0, top_k: int = 0,
+                 top_p: float = 1.0, min_p: float = 0.0) -> list:
+        """Ids: prefill the prompt, then decode one token at a time. Greedy, or
+        with `uniforms` (n_new numbers in [0, 1)) drawn by eb_sample."""
         import torch
         if len(prompt) + n_new > self.max_seq:
             raise ValueError("prompt + n_new exceeds max_seq")
+        if uniforms is None:
+            pick = lambda logits, i: int(torch.argmax(logits).item())  # noqa: E731
+        else:
+            if len(uniforms) < n_new:
+                raise ValueError("one uniform number per new token")
+            u = torch.tensor(np.asarray(uniforms, np.float32), device="cuda")
+            one = lambda v, dt: torch.tensor([v], dtype=dt, device="cuda")  # noqa: E731
+            params = self.eb.make_sample_params(one(temperature, torch.float32),
+                                                one(top_k, torch.int32), one(top_p, torch.float32),
+                                                one(min_p, torch.float32))
+            ids = torch.empty(1, dtype=torch.int32, device="cuda")
+
+            def pick(logits, i):
+                self.eb.sample(logits, params, u[i:], ids)
+                return int(ids.item())
         self.reset()
-        out = [int(torch.argmax(self.logits(list(prompt), 0)).item())]
+        out = [pick(self.logits(list(prompt), 0), 0)]
         pos = len(prompt)
         while len(out) < n_new:
-            out.append(int(torch.argmax(self.logits([out[-1]], pos)).item()))
+            out.append(pick(self.logits([out[-1]], pos), len(out)))
             pos += 1
         return out
