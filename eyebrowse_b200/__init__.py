@@ -171,10 +171,18 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_torch = None  # torch, once a call has needed it
+
+
 def _stream(stream) -> int | None:
+    global _torch
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        if _torch is None:
+            import torch
+            torch.cuda.init()
+            _torch = torch
+        # torch.cuda.current_stream() without the Stream object around it
+        return _torch._C._cuda_getCurrentRawStream(_torch._C._cuda_getDevice())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -185,9 +193,14 @@ def _check(status: int, what: str) -> None:
         raise EbError(status, what)
 
 
+_dtype_codes = {}
+
+
 def torch_dtype_code(dt) -> int:
-    import torch
-    return {torch.float32: EB_F32, torch.float16: EB_F16, torch.bfloat16: EB_BF16}[dt]
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.float32: EB_F32, torch.float16: EB_F16, torch.bfloat16: EB_BF16})
+    return _dtype_codes[dt]
 
 
 # ---------------------------------------------------------------- kernel level

@@ -5,13 +5,176 @@
 // one for V. A write finds the largest magnitude of its rows in a block, takes
 // the larger of the scale that needs and the block's own, and rounds: the new
 // rows once, the block's earlier rows again where the scale grew.
+#include <type_traits>
+
 #include "eb_kv8.cuh"
 #include "eb_rowops.cuh"
 
 namespace eb {
 
-// One CTA per (block of rows, KV head, K or V of a sequence), rows staged as
-// f32 in shared memory.
+// One CTA per (block of rows, KV head, K or V of a sequence).
+//
+// kv8_write_rows_kernel (head_dim 64, 128, 256) keeps the rows in registers
+// between finding their largest value and rounding them: a warp holds R rows,
+// E = head_dim / 32 neighbouring values of each per lane, all loaded before the
+// first is used, so every byte is read once and written once. It is bound by
+// HBM: 8192 rows of 8 heads of 128 in bf16 (50 MB) take KV8_WRITE_US us.
+// kv8_write_kernel (any other head_dim) stages them as f32 in shared memory.
+template <int E, bool E5M2>
+__device__ __forceinline__ void f8_store(uint8_t* p, const float (&v)[E], float inv) {
+  uint32_t w[(E + 3) / 4] = {};
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    w[e / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[e] * inv, v[e + 1] * inv),
+                                                   __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3)
+                << (8 * (e & 3));
+  if constexpr (E == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+  else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+  else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+// E neighbouring elements: one or two loads where `aligned`, as they lie.
+template <typename T, int E>
+struct RawRow {
+  static constexpr int W = E * (int)sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const T* p, bool aligned) {
+    if (aligned) {
+      if constexpr (W == 1) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+      } else if constexpr (W == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x;
+        w[1] = u.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+          w[i] = u.x;
+          w[i + 1] = u.y;
+          w[i + 2] = u.z;
+          w[i + 3] = u.w;
+        }
+      }
+    } else {
+      T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+      for (int i = 0; i < E; i++) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void f32(float (&f)[E]) const {
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < E; i++) f[i] = Elem<T>::to_f32(e[i]);
+  }
+};
+
+// CTAs of the same rows (K and V, every head) are neighbours: together they
+// read and write whole rows.
+template <typename T, int E, int R>
+__global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8WriteArgs a) {
+  constexpr int HD = 32 * E;
+  __shared__ float warp_max_[32];
+  const int which = blockIdx.x & 1, head = (int)((blockIdx.x >> 1) % a.hkv), b = blockIdx.y;
+  const int64_t blk0 = (blockIdx.x >> 1) / a.hkv;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t start = a.start;
+  if (a.positions) {
+    const int p = a.positions[b];
+    if (p < 0 || p > a.max_pos) return;  // an empty slot of the batch
+    start = p;
+  }
+  const int64_t end = start + a.count;
+  const int64_t blk = start / a.block + blk0;
+  const int64_t lo = max(start, blk * a.block), hi = min(end, (blk + 1) * a.block);
+  const int n = (int)(hi - lo);
+  float* scale = (which ? a.v_scale : a.k_scale) + b * a.scale_bstride + blk * a.hkv + head;
+  const int before = (int)(lo - blk * a.block);  // rows of the block in front of the new ones
+  const float old = before > 0 ? *scale : 0.f;
+
+  const T* src = static_cast<const T*>(which ? a.v : a.k) + b * a.kv_bstride + (int64_t)head * HD + lane * E;
+  const float* w = which ? a.v_norm_w : a.k_norm_w;
+  const bool turn = !which && a.cos_t;
+  // all loads first (a row past the end reads the last one again)
+  RawRow<T, E> raw[R];
+#pragma unroll
+  for (int i = 0; i < R; i++)
+    raw[i].load(src + (lo + min(i * warps + warp, n - 1) - start) * a.kv_stride, a.aligned);
+  RawRow<float, E> wr;
+  if (w) wr.load(w + lane * E, a.tables_aligned);
+  float v[R][E], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    raw[i].f32(v[i]);
+    if (w) {
+      float ss = 0.f, g[E];
+      wr.f32(g);
+#pragma unroll
+      for (int e = 0; e < E; e++) ss = __fadd_rn(ss, __fmul_rn(v[i][e], v[i][e]));
+      ss = warp_sum(ss);
+      const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+      for (int e = 0; e < E; e++) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], inv), g[e]);
+    }
+  }
+  if (turn) {
+    RawRow<float, E> tc[R], ts[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int64_t at = (lo + min(i * warps + warp, n - 1)) * (HD / 2) + (lane & 15) * E;
+      tc[i].load(a.cos_t + at, a.tables_aligned);
+      ts[i].load(a.sin_t + at, a.tables_aligned);
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      float c[E], sn[E];
+      tc[i].f32(c);
+      ts[i].f32(sn);
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[i][e], 16);
+        const float q = __fmul_rn(other, sn[e]), p = __fmul_rn(v[i][e], c[e]);
+        v[i][e] = lane < 16 ? __fsub_rn(p, q) : __fadd_rn(p, q);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++)
+#pragma unroll
+    for (int e = 0; e < E; e++) amax = f8_amax(amax, v[i][e]);
+  amax = warp_max(amax);
+  if (lane == 0) warp_max_[warp] = amax;
+  __syncthreads();  // and every thread has read the old scale
+  for (int i = 0; i < warps; i++) amax = fmaxf(amax, warp_max_[i]);
+
+  const int64_t stride = (int64_t)a.hkv * HD;
+  uint8_t* cache = static_cast<uint8_t*>(which ? a.vcache : a.kcache) + b * a.cache_bstride +
+                   (int64_t)head * HD;
+  float s = f8_need_scale(amax, a.e5m2);
+  const bool grown = before > 0 && fmaxf(s, old) != old;
+  if (before > 0) s = fmaxf(s, old);
+  const float inv = 1.0f / s, ratio = old / s;
+  uint8_t* first = cache + blk * a.block * stride + lane * E;
+  auto store = [&](auto e5m2) {
+    constexpr bool E5M2 = decltype(e5m2)::value;
+    if (grown)  // the block's earlier rows, rounded again
+      for (int r = warp; r < before; r += warps) {
+        float f[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e] = f8_decode(first[r * stride + e], E5M2);
+        f8_store<E, E5M2>(first + r * stride, f, ratio);
+      }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int r = i * warps + warp;
+      if (r < n) f8_store<E, E5M2>(first + (before + r) * stride, v[i], inv);
+    }
+  };
+  if (a.e5m2) store(std::true_type{});
+  else store(std::false_type{});
+  if (threadIdx.x == 0) *scale = s;
+}
+
 __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
   extern __shared__ float rows[];
   __shared__ float warp_max_[8];
@@ -71,17 +234,50 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
     cache[(lo + i / hd) * stride + i % hd] = f8_encode(rows[i] * inv, a.e5m2);
 }
 
-cudaError_t launch_kv8_write(const Kv8WriteArgs& a, cudaStream_t st) {
+template <typename T, int E>
+static void write_rows(const Kv8WriteArgs& a, int64_t per, cudaStream_t st) {
+  const dim3 grid((unsigned)(per * a.hkv * 2), a.batch);
+  // Rows of a warp: eight where there are enough CTAs to fill the SMs, fewer in
+  // short pieces (93 rows of 4 heads of 256, normalised: 9.1 us with eight,
+  // KV8_PIECE_US with two); a decode step's row takes one of four warps, the
+  // others are for rows that may be rounded again.
+  const int64_t ctas = per * a.hkv * 2 * a.batch;
+  if (a.count == 1) kv8_write_rows_kernel<T, E, 1><<<grid, 128, 0, st>>>(a);
+  else if (ctas >= 2 * sm_count()) kv8_write_rows_kernel<T, E, 8><<<grid, 4 * a.block, 0, st>>>(a);
+  else if (a.block <= 64) kv8_write_rows_kernel<T, E, 2><<<grid, 16 * a.block, 0, st>>>(a);
+  else kv8_write_rows_kernel<T, E, 4><<<grid, 8 * a.block, 0, st>>>(a);
+}
+
+template <typename T>
+static void write_rows_hd(const Kv8WriteArgs& a, int64_t per, cudaStream_t st) {
+  if (a.hd == 64) write_rows<T, 2>(a, per, st);
+  else if (a.hd == 128) write_rows<T, 4>(a, per, st);
+  else write_rows<T, 8>(a, per, st);
+}
+
+cudaError_t launch_kv8_write(const Kv8WriteArgs& a0, cudaStream_t st) {
+  Kv8WriteArgs a = a0;
+  const int es = a.dtype_kv == kF32 ? 4 : 2;
+  auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  a.aligned = ((bits(a.k) | bits(a.v) | (uintptr_t)(a.kv_stride * es) |
+                (uintptr_t)(a.kv_bstride * es)) & 15) == 0;
+  a.tables_aligned = ((bits(a.cos_t) | bits(a.sin_t) | bits(a.k_norm_w) | bits(a.v_norm_w)) & 15) == 0;
   const int64_t per = a.positions ? 1 : (a.start + a.count - 1) / a.block - a.start / a.block + 1;
+  if (a.hd == 64 || a.hd == 128 || a.hd == 256) {
+    if (per * a.hkv * 2 > INT32_MAX) return cudaErrorNotSupported;
+    if (a.dtype_kv == kF32) write_rows_hd<float>(a, per, st);
+    else if (a.dtype_kv == kF16) write_rows_hd<__half>(a, per, st);
+    else write_rows_hd<__nv_bfloat16>(a, per, st);
+    return cudaGetLastError();
+  }
   const int rows = (int)(a.count < a.block ? a.count : a.block);
   const size_t smem = (size_t)rows * a.hd * sizeof(float);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        kv8_write_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * 4);
+    static unsigned configured = 0;
+    const cudaError_t e = allow_smem(kv8_write_kernel, 128 * 256 * 4, &configured);
     if (e != cudaSuccess) return e;
   }
-  dim3 grid((unsigned)per, a.hkv, 2 * a.batch);
-  kv8_write_kernel<<<grid, 256, smem, st>>>(a);
+  kv8_write_kernel<<<dim3((unsigned)per, a.hkv, 2 * a.batch), 256, smem, st>>>(a);
   return cudaGetLastError();
 }
 

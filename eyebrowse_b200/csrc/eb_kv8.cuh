@@ -22,8 +22,8 @@ __device__ __forceinline__ float f8_decode(uint8_t c, bool e5m2) {
 
 // Largest magnitude that counts for a block's scale: finite values only.
 __device__ __forceinline__ float f8_amax(float m, float x) {
-  const float a = fabsf(x);
-  return a <= 3.402823466e38f ? fmaxf(m, a) : m;
+  const float a = fabsf(x);  // fmaxf passes a NaN over
+  return fmaxf(m, a <= 3.402823466e38f ? a : 0.f);
 }
 
 // The smallest power of two (2^-64 at least) with amax <= largest * scale. The
