@@ -18,85 +18,65 @@ namespace cg = cooperative_groups;
 
 namespace eb {
 
-// linear_w4_kernel multiplies on the tensor cores with mma.sync (m16n8k16,
-// f16, f32 sums): 16 weight rows by 16 inputs against 8 columns. At a few
-// columns the work is a stream of the weights, and dequantisation in
-// registers, not the matrix rate, is what a warp has to keep under its share
-// of the memory bandwidth (about 2.5 instruction slots per code and lane at
-// 6.5 TB/s); a tcgen05 operand would have to pass through shared memory
-// first, and its 128-row tiles would leave most SMs idle at decode sizes.
+// linear_w4_kernel multiplies on the tensor cores in whole numbers: mma.sync
+// m16n8k32, u8 codes by s8 activations, s32 sums. At a few rows of x the work is
+// a stream of the weights, and what a warp does per code, not the matrix rate,
+// has to keep under its share of the memory bandwidth (about 2.5 instruction
+// slots per code and lane at 6.5 TB/s). Eight codes in a word become two
+// operand registers with a shift and two ANDs; f16 operands took eleven
+// instructions (and twice the MMAs: both kinds issue at one per two clocks and
+// SM here, with k16 and k32). A tcgen05 operand would have to pass through
+// shared memory first, and its 128-row tiles would leave most SMs idle at
+// decode sizes.
 //
-// - Codes are exact in f16: 0x6400 | code is 1024 + code, 0x6400 | code << 4
-//   is 1024 + 16 code, and one subtraction or FMA leaves code - zero.
-// - The columns are f16 planes of x. Each (row of x, block of 128 inputs) is
-//   scaled by the power of two that brings its largest value to [2^14, 2^15);
-//   then a 16-bit value is one plane and an f32 value two, the second holding
-//   what the first leaves (22 bits; what falls under f16's range is below
-//   2^-39 of the block's largest). Products are exact; a group's sum is
-//   scaled by its own and the block's scale in f32 and added to the row's.
-// - The inputs of a k16 step may be any 16 as long as both operands agree, so
+// - The columns are three s8 planes of x: each (row of x, block of 128 inputs)
+//   is scaled by a power of two so that its largest value lies in [2^21, 2^22),
+//   rounded to a whole number (half a unit of f32's last place at the largest
+//   value, the only rounding), and split into bytes.
+// - A group's sum over its codes, less zero point times the sum of the same
+//   bytes, is exact in s32; it is turned to f32 (|sum| < 2^22: by adding it to
+//   the bits of 1.5 * 2^23), scaled by the group's scale and the plane's, and
+//   added to the row's f32 sum.
+// - The inputs of a k32 step may be any 32 as long as both operands agree, so
 //   the packed layout gives thread c of a quad 8 consecutive codes (one
-//   word) of each group of 32, and x is stored with its eights in the order
-//   0 4 1 5 2 6 3 7 that the words' nibble pairs come out in.
-// - The warps of a CTA: wr side by side over 32-row tiles, wk over the blocks
-//   of 128 inputs; a cluster splits the inputs further. CTAs stay and walk
-//   over the tiles, so that x is staged once and the stream of weights does
-//   not stop between tiles. Partial sums meet in shared memory, then in the
-//   cluster's.
-constexpr int kW4Ring = 3;   // blocks of a warp in its ring of shared memory
+//   word) of each group of 32, even codes in one register, odd ones in the
+//   other, and x is stored in that order.
+// - The warps of a CTA: wr side by side over 32-row tiles, wk over pairs of
+//   blocks of 128 inputs; a cluster splits the inputs further. CTAs stay and
+//   walk over the tiles, so that x is staged once and the stream of weights
+//   does not stop between tiles. Partial sums meet in shared memory, then in
+//   the cluster's.
+constexpr int kW4Ring = 2;   // pairs of blocks of a warp in its ring of shared memory
+constexpr int kW4Pair = 4096;  // bytes of a tile's pair of blocks
 constexpr int kW4Tile = 32;  // weight rows of a warp: two m16 tiles
 
-// By columns / 8. One column tile: three CTAs of 8 warps on an SM (80
-// registers a thread). More: one CTA of 16 (128), which stages x once for all.
+// By columns / 8. One column tile: two CTAs of 8 warps on an SM. More: one CTA
+// of 16, which stages x once for all.
 constexpr int w4_warps(int nt) { return nt == 1 ? 8 : 16; }
-constexpr int w4_ctas(int nt) { return nt == 1 ? 3 : 1; }
-constexpr int w4_smem(int nt) { return (nt == 1 ? 74 : 226) * 1024; }
-constexpr int w4_ring_bytes(int nt) { return w4_warps(nt) * kW4Ring * 2048; }
+constexpr int w4_ctas(int nt) { return nt == 1 ? 2 : 1; }
+constexpr int w4_smem(int nt) { return (nt == 1 ? 112 : 226) * 1024; }
+constexpr int w4_ring_bytes(int nt) { return w4_warps(nt) * kW4Ring * kW4Pair; }
 // Partial sums of a CTA's warps, one m16 tile at a time.
 constexpr int w4_red_bytes(int nt) { return w4_warps(nt) * 16 * (nt * 8 + 2) * 4; }
 
 struct W4Plan {
-  int wr, wk;      // warps of a CTA over row tiles and over input blocks
-  int split;       // CTAs of a cluster over input blocks
-  int chunk;       // blocks of 128 inputs staged at a time
-  int planes, mt;  // f16 planes per value, x rows per CTA
+  int wr, wk;      // warps of a CTA over row tiles and over pairs of input blocks
+  int split;       // CTAs of a cluster over pairs
+  int chunk;       // pairs (256 inputs) staged at a time
+  int mt;          // x rows per CTA
+  bool split_x;    // x's planes lie in the workspace
   int units;       // runs of wr tiles
   int nt, grid, smem;
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+constexpr int kW4Planes = 3;
+
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The first product of a sum.
-__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                              uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
-__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-
-// Codes 0 and 4, then 1 and 5, of a word, less the zero point, as f16 (exact).
-// bias0 = -(1024 + zero), bias1 = -(64 + zero).
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-__device__ __forceinline__ void w4_pairs(uint32_t w, uint32_t magic, __half2 bias0, __half2 bias1, uint32_t& p0,
-                                         uint32_t& p1) {
-  p0 = as_u32(__hadd2(as_half2(and_or(w, 0x000f000fu, magic)), bias0));
-  p1 = as_u32(__hfma2(as_half2(and_or(w, 0x00f000f0u, magic)), as_half2(0x2c002c00u), bias1));
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -108,10 +88,13 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Eight inputs of x row t into the planes' rows of shared memory. The 16
-// threads of a half warp hold a block of 128.
-__device__ __forceinline__ void w4_stage8(const W4Args& a, int planes, int64_t t, int64_t k0,
-                                          uint8_t* dst, int row_bytes, float* block_scale) {
+// Eight inputs of x row t into the planes' rows of shared memory (even ones,
+// then odd ones), with the block's plane scales and the groups' byte sums. The
+// 16 threads of a half warp hold a block of 128.
+template <int GROUP>
+__device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0, uint8_t* dst,
+                                          int row_bytes, float* plane_scale, int* byte_sum,
+                                          int sum_stride) {
   float f[8];
   const int64_t at = t * a.x_stride + k0;
   const char* src = static_cast<const char*>(a.x) + at * (a.dtype_x == kF32 ? 4 : 2);
@@ -121,31 +104,62 @@ __device__ __forceinline__ void w4_stage8(const W4Args& a, int planes, int64_t t
 #pragma unroll
     for (int n = 0; n < 8; n++) f[n] = k0 + n < a.in_f ? ld_any(a.x, at + n, a.dtype_x) : 0.f;
   }
-  float top = 0.f;  // of the finite values; the others go through as they are
+  float top = 0.f, odd = 0.f;  // odd: NaN if a value is not finite
 #pragma unroll
-  for (int n = 0; n < 8; n++) top = fabsf(f[n]) <= 3.402823466e38f ? fmaxf(top, fabsf(f[n])) : top;
+  for (int n = 0; n < 8; n++) {
+    top = fmaxf(top, fabsf(f[n]));
+    odd = fmaf(f[n], 0.f, odd);
+  }
   const uint32_t half = threadIdx.x & 16 ? 0xffff0000u : 0x0000ffffu;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(half, top, o));
-  const int e = max((int)(__float_as_uint(top) >> 23), 27);  // at least 2^-100
-  const float up = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
-  if ((threadIdx.x & 15) == 0) {
-    block_scale[0] = __uint_as_float((uint32_t)(e - 14) << 23);
-    if (planes == 2) block_scale[1] = block_scale[0];
+  for (int o = 8; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(half, top, o));
+    odd += __shfl_xor_sync(half, odd, o);
   }
-  uint32_t h[4], l[4];
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 27), 254);  // at least 2^-100
+  const float up = __uint_as_float((uint32_t)(127 + 21 + 127 - e) << 23);
+  uint32_t w[kW4Planes][2] = {};
 #pragma unroll
-  for (int n = 0; n < 4; n++) {
-    const float x0 = f[n] * up, x1 = f[n + 4] * up;
-    const __half2 hi = __floats2half2_rn(x0, x1);
-    const float2 hf = __half22float2(hi);
-    h[n] = as_u32(hi);
-    // an infinity or a NaN is all in the first plane
-    l[n] = pack_half2(fabsf(hf.x) <= 65504.f ? x0 - hf.x : 0.f,
-                      fabsf(hf.y) <= 65504.f ? x1 - hf.y : 0.f);
+  for (int n = 0; n < 8; n++) {
+    const int q = __float2int_rn(f[n] * up);
+    const int lo = (int)(int8_t)q, q1 = (q - lo) >> 8, mid = (int)(int8_t)q1, hi = (q1 - mid) >> 8;
+    const int sh = 8 * (n >> 1);
+    w[0][n & 1] |= (uint32_t)(uint8_t)hi << sh;
+    w[1][n & 1] |= (uint32_t)(uint8_t)mid << sh;
+    w[2][n & 1] |= (uint32_t)(uint8_t)lo << sh;
   }
-  *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-  if (planes == 2) *reinterpret_cast<uint4*>(dst + row_bytes) = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+  for (int p = 0; p < kW4Planes; p++) {
+    *reinterpret_cast<uint2*>(dst + p * row_bytes) = make_uint2(w[p][0], w[p][1]);
+    int sum = __dp4a((int)w[p][0], 0x01010101, __dp4a((int)w[p][1], 0x01010101, 0));
+#pragma unroll
+    for (int o = GROUP / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(half, sum, o);
+    if ((threadIdx.x & (GROUP / 8 - 1)) == 0) byte_sum[(threadIdx.x & 15) / (GROUP / 8) * sum_stride + p] = sum;
+    // hi counts 2^(e - 127 - 21 + 16), and so on
+    if ((threadIdx.x & 15) == 0) plane_scale[p] = __uint_as_float((uint32_t)(e - 5 - 8 * p) << 23) + odd;
+  }
+}
+
+// More than eight rows of x are split once, by w4_planes_kernel, instead of in
+// every CTA. A (row, pair of blocks) in the workspace: the planes' 256 bytes
+// each, plane scales [2 blocks][3], byte sums [2 GB groups][3], to a multiple of
+// 16 bytes.
+constexpr int w4_split_bytes(int gb) {
+  return (kW4Planes * 256 + 2 * kW4Planes * 4 * (1 + gb) + 15) / 16 * 16;
+}
+
+template <int GROUP>
+__global__ void __launch_bounds__(256) w4_planes_kernel(W4Args a) {
+  constexpr int GB = 128 / GROUP, BYTES = w4_split_bytes(GB);
+  const int64_t pairs = (a.in_f + 255) / 256;
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // a warp per (row, pair)
+  if (i >= a.m * pairs) return;
+  const int lane = threadIdx.x & 31, blk = lane >> 4, e = lane & 15;
+  uint8_t* out = static_cast<uint8_t*>(a.ws) + i * BYTES;
+  float* scales = reinterpret_cast<float*>(out + kW4Planes * 256);
+  w4_stage8<GROUP>(a, i / pairs, (i % pairs) * 256 + lane * 8,
+                   out + blk * 128 + (e & 3) * 32 + (e >> 2) * 8, 256, scales + blk * kW4Planes,
+                   reinterpret_cast<int*>(scales + 2 * kW4Planes) + blk * GB * kW4Planes, kW4Planes);
 }
 
 __device__ __forceinline__ float w4_scale(uint32_t bits, bool bf16) {
@@ -160,71 +174,90 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
   float* red = reinterpret_cast<float*>(smem_raw + w4_ring_bytes(NT));  // [warps][16][LD]
   const int cta_rows = pl.wr * kW4Tile;
   float* part = red + w4_red_bytes(NT) / 4;  // [2][mt][cta_rows], with a cluster
-  float* xscale = part + (pl.split > 1 ? 2 * pl.mt * cta_rows : 0);  // [chunk][8 NT]: of a block's columns
-  uint8_t* zeros = reinterpret_cast<uint8_t*>(xscale + pl.chunk * NT * 8);  // what columns past the last read
+  // of a block's columns: plane scales [2 chunk][8 NT], a group's byte sums [2 chunk GB][8 NT]
+  float* xscale = part + (pl.split > 1 ? 2 * pl.mt * cta_rows : 0);
+  int* xsum = reinterpret_cast<int*>(xscale + 2 * pl.chunk * NT * 8);
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + 2 * pl.chunk * GB * NT * 8);  // what columns past the last read
   uint8_t* xs = zeros + 256;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, n = lane >> 2;
   const int wk = warp % pl.wk, wr = warp / pl.wk;
   const int rank = blockIdx.x % pl.split;
   const int64_t m0 = (int64_t)blockIdx.y * pl.mt;
   const int mt = (int)min((int64_t)pl.mt, a.m - m0);
-  const int P = pl.planes, cols = mt * P;
+  constexpr int P = kW4Planes;
+  const int cols = mt * P;
   const int out_f = (int)a.out_f;
   const int blocks = (int)((a.in_f + 127) / 128), groups = (int)((a.in_f + GROUP - 1) / GROUP);
-  const int kb0 = (int)((int64_t)blocks * rank / pl.split);
-  const int kb1 = (int)((int64_t)blocks * (rank + 1) / pl.split);
-  const int row_bytes = pl.chunk * 256 + 64;  // 64 past a multiple of 128: no bank is hit twice
+  const int pairs = (blocks + 1) / 2;
+  const int p0 = (int)((int64_t)pairs * rank / pl.split);
+  const int p1 = (int)((int64_t)pairs * (rank + 1) / pl.split);
+  const int row_bytes = pl.chunk * 256 + 16;  // 16 past a multiple of 128: no bank is hit twice
   const uint16_t* scale = static_cast<const uint16_t*>(a.scale);
   const bool sbf = a.dtype_scale == kBF16;
   const int step = gridDim.x / pl.split;
 
-  // The warp's blocks, tile after tile, pass through a ring of its own, each
-  // thread reading back what it copied: no barrier, and several blocks of
-  // every warp in flight without registers. Thread: rows n, n + 8, n + 16 and
-  // n + 24 of the tile (the last row again past the end), 16 bytes of each.
-  // The scales (low half) and zero points of a block's groups come with it,
+  // The warp's pairs, tile after tile, pass through a ring of its own, each
+  // thread reading back what it copied: no barrier, and two pairs of every
+  // warp in flight without registers. Thread: rows n, n + 8, n + 16 and n + 24
+  // of the tile (the last row again past the end), 16 bytes of each block. The
+  // scales (low half) and zero points of a pair's groups come one pair ahead,
   // row `lane` of the tile in a thread.
   struct Meta {
-    uint32_t v[GB];
+    uint32_t v[2 * GB];
   };
-  const uint32_t ring = smem_u32(smem_raw) + warp * kW4Ring * 2048 + lane * 16;
-  int fetch_unit = blockIdx.x / pl.split, fetch_kb = kb0 + wk, fetch_slot = 0, fetch_row = 0;
+  const uint32_t ring = smem_u32(smem_raw) + warp * kW4Ring * kW4Pair + lane * 16;
+  const uint8_t* ring_p = smem_raw + warp * kW4Ring * kW4Pair + lane * 16;
+  int fetch_unit = blockIdx.x / pl.split, fetch_p = p0 + wk;
   const uint8_t* from[4];
   auto aim = [&]() {
     const int row0 = (fetch_unit * pl.wr + wr) * kW4Tile;
-    fetch_row = min(row0 + lane, out_f - 1);
 #pragma unroll
     for (int j = 0; j < 4; j++)
-      from[j] = static_cast<const uint8_t*>(a.q) + (int64_t)min(row0 + n + 8 * j, out_f - 1) * blocks * 64 + c * 16;
+      from[j] = static_cast<const uint8_t*>(a.q) + (int64_t)min(row0 + n + 8 * j, out_f - 1) * blocks * 64 +
+                c * 16 + fetch_p * 128;
   };
-  auto fetch = [&](Meta& meta) {
-    if (fetch_unit < pl.units && fetch_kb < kb1) {
+  auto fetch = [&](int slot) {
+    if (fetch_unit < pl.units && fetch_p < p1) {
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        cp_async16(ring + fetch_slot * 2048 + j * 512, from[j] + (uint32_t)(fetch_kb * 64));
+      for (int j = 0; j < 4; j++) cp_async16(ring + slot * kW4Pair + j * 512, from[j]);
+      if (2 * fetch_p + 1 < blocks)  // an odd last block has no partner: x is zero there
 #pragma unroll
-      for (int g = 0; g < GB; g++) {
-        const int64_t at = (int64_t)min(fetch_kb * GB + g, groups - 1) * out_f + fetch_row;
-        meta.v[g] = (uint32_t)__ldg(scale + at) | (a.zero ? (uint32_t)__ldg(a.zero + at) : 8u) << 16;
-      }
-      fetch_kb += pl.wk;
-      if (fetch_kb >= kb1) {
-        fetch_kb = kb0 + wk;
+        for (int j = 0; j < 4; j++) cp_async16(ring + slot * kW4Pair + 2048 + j * 512, from[j] + 64);
+#pragma unroll
+      for (int j = 0; j < 4; j++) from[j] += pl.wk * 128;
+      fetch_p += pl.wk;
+      if (fetch_p >= p1) {
+        fetch_p = p0 + wk;
         fetch_unit += step;
         aim();
       }
     }
     cp_async_commit();
-    fetch_slot = fetch_slot + 1 == kW4Ring ? 0 : fetch_slot + 1;
   };
-  for (int i = threadIdx.x; i < pl.chunk * NT * 8 + 64; i += THREADS) xscale[i] = 0.f;  // and zeros
-  uint32_t magic = 0x64006400u;
-  asm volatile("" : "+r"(magic));  // in a register: LOP3 takes one immediate
-  static_assert(kW4Ring == 3, "two blocks ahead: meta0 and meta1");
-  Meta meta0{}, meta1{};
+  int meta_unit = fetch_unit, meta_p = fetch_p;
+  auto fetch_meta = [&](Meta& meta) {
+    if (meta_unit < pl.units && meta_p < p1) {
+      const int row = min((meta_unit * pl.wr + wr) * kW4Tile + lane, out_f - 1);
+#pragma unroll
+      for (int g = 0; g < 2 * GB; g++) {
+        const int64_t at = (int64_t)min(meta_p * 2 * GB + g, groups - 1) * out_f + row;
+        meta.v[g] = (uint32_t)__ldg(scale + at) | (a.zero ? (uint32_t)__ldg(a.zero + at) : 8u) << 16;
+      }
+      meta_p += pl.wk;
+      if (meta_p >= p1) {
+        meta_p = p0 + wk;
+        meta_unit += step;
+      }
+    }
+  };
+  Meta ahead{};
   aim();
-  fetch(meta0);
-  fetch(meta1);
+#pragma unroll
+  for (int d = 0; d < kW4Ring; d++) fetch(d);
+  fetch_meta(ahead);
+  for (int i = threadIdx.x; i < 2 * pl.chunk * NT * 8 * (1 + GB) + 64; i += THREADS)
+    xscale[i] = 0.f;  // and xsum, and zeros
+  constexpr int kMagic = 0x4b400000;  // 1.5 * 2^23: adding |v| < 2^22 gives the float 1.5 * 2^23 + v
 
   int slot = 0, buf = 0;
   for (int unit = blockIdx.x / pl.split; unit < pl.units; unit += step) {
@@ -236,91 +269,126 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[rt][t][e] = 0.f;
 
-    for (int ch = kb0; ch < kb1; ch += pl.chunk) {
-      const int end = min(ch + pl.chunk, kb1);
-      if (ch > kb0 || unit == blockIdx.x / pl.split || pl.chunk < kb1 - kb0) {
+    for (int ch = p0; ch < p1; ch += pl.chunk) {
+      const int end = min(ch + pl.chunk, p1);
+      if (ch > p0 || unit == blockIdx.x / pl.split || pl.chunk < p1 - p0) {
         __syncthreads();  // what was staged before has been read
-        const int eights = (end - ch) * 16;
+        const int eights = (end - ch) * 32;
+        if (pl.split_x) {
+          constexpr int BYTES = w4_split_bytes(GB), SCALES = 2 * P, SUMS = 2 * GB * P;
+          const uint8_t* src = static_cast<const uint8_t*>(a.ws) + (m0 * pairs + ch) * BYTES;
+          const int n_pairs = end - ch, words = P * 16;
+          for (int i = threadIdx.x; i < mt * n_pairs * words; i += THREADS) {
+            const int word = i % words, q = i / words, t = q / n_pairs, pr = q % n_pairs;
+            *reinterpret_cast<uint4*>(xs + (t * P + word / 16) * row_bytes + pr * 256 + word % 16 * 16) =
+                __ldg(reinterpret_cast<const uint4*>(src + ((int64_t)t * pairs + pr) * BYTES) + word);
+          }
+          for (int i = threadIdx.x; i < mt * n_pairs * (SCALES + SUMS); i += THREADS) {
+            const int j = i % (SCALES + SUMS), q = i / (SCALES + SUMS), t = q / n_pairs, pr = q % n_pairs;
+            const int v = __ldg(reinterpret_cast<const int*>(src + ((int64_t)t * pairs + pr) * BYTES + P * 256) + j);
+            if (j < SCALES) xscale[(pr * 2 + j / P) * NT * 8 + t * P + j % P] = __int_as_float(v);
+            else xsum[(pr * 2 * GB + (j - SCALES) / P) * NT * 8 + t * P + (j - SCALES) % P] = v;
+          }
+        } else
         for (int i = threadIdx.x; i < eights * mt; i += THREADS) {
           const int t = i / eights, e = i % eights;
-          w4_stage8(a, P, m0 + t, (int64_t)ch * 128 + e * 8, xs + t * P * row_bytes + e * 16,
-                    row_bytes, &xscale[(e >> 4) * NT * 8 + t * P]);
+          w4_stage8<GROUP>(a, m0 + t, (int64_t)ch * 256 + e * 8,
+                           xs + t * P * row_bytes + (e >> 4) * 128 + (e & 3) * 32 + ((e >> 2) & 3) * 8,
+                           row_bytes, &xscale[(e >> 4) * NT * 8 + t * P],
+                           &xsum[(e >> 4) * GB * NT * 8 + t * P], NT * 8);
         }
         __syncthreads();
       }
-      for (int kb = ch + wk; kb < end; kb += pl.wk) {
-        cp_async_wait<kW4Ring - 2>();
-        uint4 w[4];
+      for (int p = ch + wk; p < end; p += pl.wk) {
+        cp_async_wait<kW4Ring - 1>();
+        // With one column tile both blocks' words are in registers at once; with
+        // more there is room for one block's.
+        constexpr int KW = NT == 1 ? 2 : 1;
+        uint4 w[KW][4];
+        auto read = [&](int k) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          w[j] = *reinterpret_cast<const uint4*>(smem_raw + (warp * kW4Ring + slot) * 2048 + j * 512 + lane * 16);
-        slot = slot + 1 == kW4Ring ? 0 : slot + 1;
-        const Meta meta = meta0;
-        meta0 = meta1;
-        fetch(meta1);
-        const uint8_t* xb[NT];  // column 8 t + n, word 0
+          for (int j = 0; j < 4; j++)
+            w[k % KW][j] = *reinterpret_cast<const uint4*>(ring_p + slot * kW4Pair + k * 2048 + j * 512);
+          if (k == 1) fetch(slot);  // into the place just read
+        };
+        const Meta meta = ahead;
+        fetch_meta(ahead);
+        const uint8_t* xb[NT];  // column 8 t + n, words 0 and 1
 #pragma unroll
         for (int t = 0; t < NT; t++)
-          xb[t] = (8 * t + n < cols ? xs + (8 * t + n) * row_bytes + (kb - ch) * 256 : zeros) + c * 16;
-        // Chains of dependent products are kept short: a sum per m16 tile and,
-        // at one column tile, per half of a word.
-        constexpr int H = NT == 1 ? 2 : 1;
-        float sum[2][NT][H][4];
-        __half2 bias[2][2][2];
-        float s[2][2];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const bool first = i * 32 % GROUP == 0, last = (i + 1) * 32 % GROUP == 0;
-          if (first) {
-#pragma unroll
-            for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-              for (int r = 0; r < 2; r++) {
-                const uint32_t m = __shfl_sync(0xffffffffu, meta.v[i * 32 / GROUP], n + 16 * rt + 8 * r);
-                s[rt][r] = w4_scale(m & 0xffffu, sbf);
-                // -(1024 + z) and -(64 + z) in both halves: z is one, or 16, units of the last place
-                bias[rt][r][0] = as_half2(((m >> 16) | 0xe400u) * 0x10001u);
-                bias[rt][r][1] = as_half2((((m >> 12) & 0xf0u) | 0xd400u) * 0x10001u);
-              }
-          }
+          xb[t] = (8 * t + n < cols ? xs + (8 * t + n) * row_bytes + (p - ch) * 256 : zeros) + c * 32;
+        const float* bs = xscale + (p - ch) * 2 * NT * 8 + 2 * c;
+        const int* bz = xsum + (p - ch) * 2 * GB * NT * 8 + 2 * c;
+        // Two words of one block: 64 inputs of both m16 tiles.
+        auto words = [&](int k, int i2, int (&sum)[2][NT][4]) {
           uint4 x[NT];
 #pragma unroll
-          for (int t = 0; t < NT; t++) x[t] = *reinterpret_cast<const uint4*>(xb[t] + i * 64);
+          for (int t = 0; t < NT; t++) x[t] = *reinterpret_cast<const uint4*>(xb[t] + k * 128 + i2 * 16);
 #pragma unroll
-          for (int rt = 0; rt < 2; rt++) {
-            const uint4 w0 = w[2 * rt], w1 = w[2 * rt + 1];
-            const uint32_t u0 = i == 0 ? w0.x : i == 1 ? w0.y : i == 2 ? w0.z : w0.w;
-            const uint32_t u1 = i == 0 ? w1.x : i == 1 ? w1.y : i == 2 ? w1.z : w1.w;
-            uint32_t f0[4], f1[4];
-            w4_pairs(u0, magic, bias[rt][0][0], bias[rt][0][1], f0[0], f0[2]);
-            w4_pairs(u1, magic, bias[rt][1][0], bias[rt][1][1], f0[1], f0[3]);
-            w4_pairs(u0 >> 8, magic, bias[rt][0][0], bias[rt][0][1], f1[0], f1[2]);
-            w4_pairs(u1 >> 8, magic, bias[rt][1][0], bias[rt][1][1], f1[1], f1[3]);
+          for (int h = 0; h < 2; h++) {
+            const int i = 2 * i2 + h;
+            const bool first = i * 32 % GROUP == 0, last = (i + 1) * 32 % GROUP == 0;
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-              if (first) mma_f16_first(sum[rt][t][0], f0, x[t].x, x[t].y);
-              else mma_f16(sum[rt][t][0], f0, x[t].x, x[t].y);
+            for (int rt = 0; rt < 2; rt++) {
+              const uint4 w0 = w[k % KW][2 * rt], w1 = w[k % KW][2 * rt + 1];
+              const uint32_t u0 = i == 0 ? w0.x : i == 1 ? w0.y : i == 2 ? w0.z : w0.w;
+              const uint32_t u1 = i == 0 ? w1.x : i == 1 ? w1.y : i == 2 ? w1.z : w1.w;
+              const uint32_t f[4] = {u0 & 0x0f0f0f0fu, u1 & 0x0f0f0f0fu, (u0 >> 4) & 0x0f0f0f0fu,
+                                     (u1 >> 4) & 0x0f0f0f0fu};
+#pragma unroll
+              for (int t = 0; t < NT; t++) {
+                if (first)
+#pragma unroll
+                  for (int e = 0; e < 4; e++) sum[rt][t][e] = kMagic;
+                mma_u8s8(sum[rt][t], f, h ? x[t].z : x[t].x, h ? x[t].w : x[t].y);
+              }
             }
+            if (last) {
+              const int g = k * GB + i * 32 / GROUP;
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-              if (first && H == 2) mma_f16_first(sum[rt][t][H - 1], f1, x[t].z, x[t].w);
-              else mma_f16(sum[rt][t][H - 1], f1, x[t].z, x[t].w);
+              for (int rt = 0; rt < 2; rt++) {
+                float s[2];
+                int z[2];
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                  const uint32_t m = __shfl_sync(0xffffffffu, meta.v[g], n + 16 * rt + 8 * r);
+                  s[r] = w4_scale(m & 0xffffu, sbf);
+                  z[r] = (int)(m >> 16);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                  const float2 b2 = *reinterpret_cast<const float2*>(bs + k * NT * 8 + 8 * t);
+                  const int2 z2 = *reinterpret_cast<const int2*>(bz + g * NT * 8 + 8 * t);
+#pragma unroll
+                  for (int e = 0; e < 4; e++) {
+                    const int v = sum[rt][t][e] - z[e >> 1] * (e & 1 ? z2.y : z2.x);
+                    acc[rt][t][e] = fmaf(__int_as_float(v) - 12582912.f, s[e >> 1] * (e & 1 ? b2.y : b2.x),
+                                         acc[rt][t][e]);
+                  }
+                }
+              }
             }
           }
-          if (last) {
+        };
+        if constexpr (NT == 1) {
+          // both blocks abreast: four chains of dependent products
+          int sum[2][2][NT][4];
+          read(0);
+          read(1);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-              const float2 xb2 = *reinterpret_cast<const float2*>(xscale + (kb - ch) * NT * 8 + 8 * t + 2 * c);
+          for (int i2 = 0; i2 < 2; i2++)
 #pragma unroll
-              for (int rt = 0; rt < 2; rt++)
+            for (int k = 0; k < 2; k++) words(k, i2, sum[k]);
+        } else {
+          int sum[2][NT][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  const float v = H == 2 ? sum[rt][t][0][e] + sum[rt][t][H - 1][e] : sum[rt][t][0][e];
-                  acc[rt][t][e] = fmaf(v * s[rt][e >> 1], e & 1 ? xb2.y : xb2.x, acc[rt][t][e]);
-                }
-            }
+          for (int k = 0; k < 2; k++) {
+            read(k);
+#pragma unroll
+            for (int i2 = 0; i2 < 2; i2++) words(k, i2, sum);
           }
         }
+        slot ^= 1;
       }
     }
 
@@ -342,7 +410,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
         float v = 0.f;
         for (int k = 0; k < pl.wk; k++) {
           const float* s = red + ((w * pl.wk + k) * 16 + rr) * LD + t * P;
-          v += P == 2 ? s[1] + s[0] : s[0];
+          v += (s[2] + s[1]) + s[0];
         }
         const int row = w * kW4Tile + rt * 16 + rr;
         if (pl.split > 1) part[(buf * pl.mt + t) * cta_rows + row] = v;
@@ -369,37 +437,50 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
   if (pl.split > 1) cg::this_cluster().sync();  // no CTA leaves while its sums are read
 }
 
-size_t linear_w4_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+// Rows of x that a CTA multiplies at once, evened out over the passes.
+constexpr int kW4Rows = 24 / kW4Planes;
+static int w4_pass_rows(int64_t m) {
+  const int64_t passes = (m + kW4Rows - 1) / kW4Rows;
+  return (int)((m + passes - 1) / passes);
+}
+static int w4_column_tiles(int64_t m) { return (w4_pass_rows(m) * kW4Planes + 7) / 8; }
+
+size_t linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t) {
+  if (m <= kW4Rows) return 0;
+  return ((size_t)m * (size_t)((in_f + 255) / 256) * w4_split_bytes(4) + 255) / 256 * 256;  // any group
+}
 
 // The shape of a launch: of every (wk, split) whose staged x fits, the one
-// with the least work on the busiest SM, counted in blocks of 128 inputs of
-// one warp (an eight of x staged by each thread is about a quarter, a tile's
-// sums about one, a cluster's about another), and at least what the longest
-// row of blocks of one warp takes (a warp alone takes about as long for a
-// block as a full SM for 24).
-static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int planes) {
+// with the least work on the busiest SM, counted in pairs of blocks of one warp
+// (about 480 instructions; an eight of x staged by each thread is about a
+// third of that, copied a twentieth, a tile's sums about a third, a cluster's
+// about another), and at least
+// what the longest row of pairs of one warp takes (a warp alone takes about as
+// long for a pair as a full SM for 16). limit[split]: clusters of that size that
+// are resident at once (an SM group holds whole clusters only: 148 SMs do not
+// hold 21 clusters of 7).
+static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int* limit) {
   W4Plan p{};
-  p.planes = planes;
-  const int64_t most = 24 / planes, passes = (m + most - 1) / most;
-  p.mt = (int)((m + passes - 1) / passes);
-  const int cols = p.mt * planes;
-  p.nt = (cols + 7) / 8;
-  const int64_t tiles = (out_f + kW4Tile - 1) / kW4Tile, blocks = (in_f + 127) / 128;
-  const int64_t slots = (int64_t)w4_ctas(p.nt) * sm_count();
+  const int64_t passes = (m + kW4Rows - 1) / kW4Rows;
+  p.mt = w4_pass_rows(m);
+  p.split_x = m > kW4Rows;
+  const int cols = p.mt * kW4Planes;
+  p.nt = w4_column_tiles(m);
+  const int64_t tiles = (out_f + kW4Tile - 1) / kW4Tile, pairs = (in_f + 255) / 256;
   const int warps = w4_warps(p.nt);
   const int fixed = w4_ring_bytes(p.nt) + w4_red_bytes(p.nt);
   double best = 0;
   for (int wk = warps; wk >= 1; wk /= 2)
-    for (int split = 1; split <= 8 && split <= blocks; split++) {
+    for (int split = 1; split <= 8 && split <= pairs; split++) {
       const int wr = warps / wk;
       const int part = split > 1 ? 2 * p.mt * wr * kW4Tile * 4 : 0;
-      const int64_t range = (blocks + split - 1) / split;
-      const int64_t left = w4_smem(p.nt) - fixed - part - 64 * cols - 256;
-      const int64_t fit = std::max<int64_t>(left, 0) / (256 * cols + 32 * p.nt) / wk * wk;
+      const int64_t range = (pairs + split - 1) / split;
+      const int64_t left = w4_smem(p.nt) - fixed - part - 16 * cols - 256;
+      const int64_t fit = std::max<int64_t>(left, 0) / (256 * cols + 64 * p.nt * (1 + gb)) / wk * wk;
       if (fit == 0) continue;  // chunks are whole turns of the wk warps
       const int64_t chunk = std::min(range, fit);
       const int64_t units = (tiles + wr - 1) / wr;
-      const int64_t clusters = std::max<int64_t>(1, slots / passes / split);
+      const int64_t clusters = std::max<int64_t>(1, limit[split] / passes);
       const int64_t grid = std::min(units, clusters) * split;
       const int64_t turns = (units + clusters - 1) / clusters;
       // an SM's CTAs; at most one of them has the last turn if few have
@@ -407,11 +488,11 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int planes) {
       const int64_t last = (units - (turns - 1) * clusters) * split * passes;
       const int64_t unit_sm = last <= sm_count() ? per_sm * (turns - 1) + 1 : per_sm * turns;
       const double blocks_warp = (double)((range + wk - 1) / wk);
-      const double stage = 0.25 * (double)((range * 16 * p.mt + warps * 32 - 1) / (warps * 32));
-      const double sums = split > 1 ? 2 : 1;
+      const double stage = (p.split_x ? 0.06 : 0.3) * (double)((range * 32 * p.mt + warps * 32 - 1) / (warps * 32));
+      const double sums = split > 1 ? 0.6 : 0.3;
       const double staged = chunk < range ? unit_sm * stage : per_sm * stage;
       const double busy = warps * (unit_sm * (blocks_warp + sums) + staged);
-      const double alone = 24.0 * (turns * (blocks_warp + sums) + (chunk < range ? turns : 1) * stage);
+      const double alone = 16.0 * (turns * (blocks_warp + sums) + (chunk < range ? turns : 1) * stage);
       const double cost = std::max(busy, alone);
       if (best == 0 || cost < best) {
         best = cost;
@@ -421,18 +502,53 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int planes) {
         p.chunk = (int)chunk;
         p.units = (int)units;
         p.grid = (int)grid;
-        p.smem = fixed + part + (int)chunk * 32 * p.nt + 256 + cols * (int)(chunk * 256 + 64);
+        p.smem = fixed + part + (int)chunk * 64 * p.nt * (1 + gb) + 256 + cols * (int)(chunk * 256 + 16);
       }
     }
   return p;
 }
 
+// Resident clusters of every size, asked of the runtime once per kernel.
 template <int NT, int GROUP>
-static cudaError_t run_w4(const W4Args& a, const W4Plan& p, cudaStream_t st) {
+static cudaError_t w4_limits(int (&limit)[9]) {
+  static int cache[9] = {};
+  auto kern = linear_w4_kernel<NT, GROUP>;
+  for (int split = 1; split <= 8; split++) {
+    limit[split] = __atomic_load_n(&cache[split], __ATOMIC_RELAXED);
+    if (limit[split] > 0) continue;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(split);
+    cfg.blockDim = dim3(w4_warps(NT) * 32);
+    cfg.dynamicSmemBytes = w4_smem(NT);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&limit[split], kern, &cfg);
+    if (e != cudaSuccess) return e;
+    if (limit[split] < 1) limit[split] = 1;
+    __atomic_store_n(&cache[split], limit[split], __ATOMIC_RELAXED);
+  }
+  return cudaSuccess;
+}
+
+template <int NT, int GROUP>
+static cudaError_t run_w4(const W4Args& a, cudaStream_t st) {
   auto kern = linear_w4_kernel<NT, GROUP>;
   static unsigned configured = 0;  // a bit per device
-  const cudaError_t e = allow_smem(kern, w4_smem(NT), &configured);
+  cudaError_t e = allow_smem(kern, w4_smem(NT), &configured);
+  int limit[9];
+  if (e == cudaSuccess) e = w4_limits<NT, GROUP>(limit);
   if (e != cudaSuccess) return e;
+  const W4Plan p = plan_w4(a.m, a.in_f, a.out_f, 128 / GROUP, limit);
+  if (p.split_x) {
+    const int64_t warps = a.m * ((a.in_f + 255) / 256);
+    w4_planes_kernel<GROUP><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)p.grid, (unsigned)((a.m + p.mt - 1) / p.mt));
   cfg.blockDim = dim3(w4_warps(NT) * 32);
@@ -448,20 +564,19 @@ static cudaError_t run_w4(const W4Args& a, const W4Plan& p, cudaStream_t st) {
 }
 
 template <int GROUP>
-static cudaError_t run_w4_nt(const W4Args& a, const W4Plan& p, cudaStream_t st) {
-  switch (p.nt) {
-    case 1: return run_w4<1, GROUP>(a, p, st);
-    case 2: return run_w4<2, GROUP>(a, p, st);
-    default: return run_w4<3, GROUP>(a, p, st);
+static cudaError_t run_w4_nt(const W4Args& a, cudaStream_t st) {
+  switch (w4_column_tiles(a.m)) {
+    case 1: return run_w4<1, GROUP>(a, st);
+    case 2: return run_w4<2, GROUP>(a, st);
+    default: return run_w4<3, GROUP>(a, st);
   }
 }
 
 cudaError_t launch_linear_w4(const W4Args& a, cudaStream_t st) {
-  const W4Plan p = plan_w4(a.m, a.in_f, a.out_f, a.dtype_x == kF32 ? 2 : 1);
   switch (a.group) {
-    case 32: return run_w4_nt<32>(a, p, st);
-    case 64: return run_w4_nt<64>(a, p, st);
-    default: return run_w4_nt<128>(a, p, st);
+    case 32: return run_w4_nt<32>(a, st);
+    case 64: return run_w4_nt<64>(a, st);
+    default: return run_w4_nt<128>(a, st);
   }
 }
 
