@@ -89,11 +89,12 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 
 // Eight inputs of x row t into the planes' rows of shared memory (even ones,
-// then odd ones), with the block's plane scales and the groups' byte sums. The
-// 16 threads of a half warp hold a block of 128.
-template <int GROUP>
+// then odd ones). The 16 threads of a half warp hold a block of 128. With it
+// the block's scales and the groups' sums: of each plane (three numbers each;
+// the sums are whole), or of the whole numbers (JOINT: one each, floats).
+template <int GROUP, bool JOINT>
 __device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0, uint8_t* dst,
-                                          int row_bytes, float* plane_scale, int* byte_sum,
+                                          int row_bytes, float* scale, float* sums,
                                           int sum_stride) {
   float f[8];
   const int64_t at = t * a.x_stride + k0;
@@ -128,25 +129,35 @@ __device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0
     w[1][n & 1] |= (uint32_t)(uint8_t)mid << sh;
     w[2][n & 1] |= (uint32_t)(uint8_t)lo << sh;
   }
+  const int lane = threadIdx.x & 15;
+  int sum[kW4Planes];
 #pragma unroll
   for (int p = 0; p < kW4Planes; p++) {
     *reinterpret_cast<uint2*>(dst + p * row_bytes) = make_uint2(w[p][0], w[p][1]);
-    int sum = __dp4a((int)w[p][0], 0x01010101, __dp4a((int)w[p][1], 0x01010101, 0));
+    sum[p] = __dp4a((int)w[p][0], 0x01010101, __dp4a((int)w[p][1], 0x01010101, 0));
 #pragma unroll
-    for (int o = GROUP / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(half, sum, o);
-    if ((threadIdx.x & (GROUP / 8 - 1)) == 0) byte_sum[(threadIdx.x & 15) / (GROUP / 8) * sum_stride + p] = sum;
-    // hi counts 2^(e - 127 - 21 + 16), and so on
-    if ((threadIdx.x & 15) == 0) plane_scale[p] = __uint_as_float((uint32_t)(e - 5 - 8 * p) << 23) + odd;
+    for (int o = GROUP / 16; o > 0; o >>= 1) sum[p] += __shfl_xor_sync(half, sum[p], o);
+  }
+  // hi counts 2^(e - 127 - 21 + 16), and so on
+  auto unit = [&](int p) { return __uint_as_float((uint32_t)(e - 5 - 8 * p) << 23) + odd; };
+  float* at_group = sums + lane / (GROUP / 8) * sum_stride;
+  if constexpr (JOINT) {
+    if (lane % (GROUP / 8) == 0)
+      *at_group = fmaf((float)sum[0], 65536.f, fmaf((float)sum[1], 256.f, (float)sum[2]));
+    if (lane == 0) *scale = unit(2);
+  } else {
+#pragma unroll
+    for (int p = 0; p < kW4Planes; p++) {
+      if (lane % (GROUP / 8) == 0) at_group[p] = __int_as_float(sum[p]);
+      if (lane == 0) scale[p] = unit(p);
+    }
   }
 }
 
 // More than eight rows of x are split once, by w4_planes_kernel, instead of in
 // every CTA. A (row, pair of blocks) in the workspace: the planes' 256 bytes
-// each, plane scales [2 blocks][3], byte sums [2 GB groups][3], to a multiple of
-// 16 bytes.
-constexpr int w4_split_bytes(int gb) {
-  return (kW4Planes * 256 + 2 * kW4Planes * 4 * (1 + gb) + 15) / 16 * 16;
-}
+// each, the blocks' two scales, the groups' 2 GB sums, to a multiple of 16 bytes.
+constexpr int w4_split_bytes(int gb) { return (kW4Planes * 256 + 2 * 4 * (1 + gb) + 15) / 16 * 16; }
 
 template <int GROUP>
 __global__ void __launch_bounds__(256) w4_planes_kernel(W4Args a) {
@@ -157,9 +168,9 @@ __global__ void __launch_bounds__(256) w4_planes_kernel(W4Args a) {
   const int lane = threadIdx.x & 31, blk = lane >> 4, e = lane & 15;
   uint8_t* out = static_cast<uint8_t*>(a.ws) + i * BYTES;
   float* scales = reinterpret_cast<float*>(out + kW4Planes * 256);
-  w4_stage8<GROUP>(a, i / pairs, (i % pairs) * 256 + lane * 8,
-                   out + blk * 128 + (e & 3) * 32 + (e >> 2) * 8, 256, scales + blk * kW4Planes,
-                   reinterpret_cast<int*>(scales + 2 * kW4Planes) + blk * GB * kW4Planes, kW4Planes);
+  w4_stage8<GROUP, true>(a, i / pairs, (i % pairs) * 256 + lane * 8,
+                         out + blk * 128 + (e & 3) * 32 + (e >> 2) * 8, 256, scales + blk,
+                         scales + 2 + blk * GB, 1);
 }
 
 __device__ __forceinline__ float w4_scale(uint32_t bits, bool bf16) {
@@ -174,10 +185,15 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
   float* red = reinterpret_cast<float*>(smem_raw + w4_ring_bytes(NT));  // [warps][16][LD]
   const int cta_rows = pl.wr * kW4Tile;
   float* part = red + w4_red_bytes(NT) / 4;  // [2][mt][cta_rows], with a cluster
-  // of a block's columns: plane scales [2 chunk][8 NT], a group's byte sums [2 chunk GB][8 NT]
+  // Columns: one or two tiles hold the planes of each row of x side by side
+  // (3 t + p). Three hold a plane each (8 p + t), so that a thread has all
+  // planes of its two rows and joins them before it scales.
+  constexpr bool JOINT = NT == 3;
+  constexpr int XC = JOINT ? 8 : NT * 8;
+  // of a block's columns: scales [2 chunk][XC], a group's sums [2 chunk GB][XC]
   float* xscale = part + (pl.split > 1 ? 2 * pl.mt * cta_rows : 0);
-  int* xsum = reinterpret_cast<int*>(xscale + 2 * pl.chunk * NT * 8);
-  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + 2 * pl.chunk * GB * NT * 8);  // what columns past the last read
+  float* xsum = xscale + 2 * pl.chunk * XC;
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + 2 * pl.chunk * GB * XC);  // what columns past the last read
   uint8_t* xs = zeros + 256;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, n = lane >> 2;
   const int wk = warp % pl.wk, wr = warp / pl.wk;
@@ -185,7 +201,8 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
   const int64_t m0 = (int64_t)blockIdx.y * pl.mt;
   const int mt = (int)min((int64_t)pl.mt, a.m - m0);
   constexpr int P = kW4Planes;
-  const int cols = mt * P;
+  auto column = [&](int t, int p) { return JOINT ? 8 * p + t : t * P + p; };
+  auto has_column = [&](int t) { return JOINT ? n < mt : 8 * t + n < mt * P; };  // 8 t + n
   const int out_f = (int)a.out_f;
   const int blocks = (int)((a.in_f + 127) / 128), groups = (int)((a.in_f + GROUP - 1) / GROUP);
   const int pairs = (blocks + 1) / 2;
@@ -255,17 +272,18 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
 #pragma unroll
   for (int d = 0; d < kW4Ring; d++) fetch(d);
   fetch_meta(ahead);
-  for (int i = threadIdx.x; i < 2 * pl.chunk * NT * 8 * (1 + GB) + 64; i += THREADS)
+  for (int i = threadIdx.x; i < 2 * pl.chunk * XC * (1 + GB) + 64; i += THREADS)
     xscale[i] = 0.f;  // and xsum, and zeros
   constexpr int kMagic = 0x4b400000;  // 1.5 * 2^23: adding |v| < 2^22 gives the float 1.5 * 2^23 + v
 
   int slot = 0, buf = 0;
   for (int unit = blockIdx.x / pl.split; unit < pl.units; unit += step) {
-    float acc[2][NT][4];
+    constexpr int AT = JOINT ? 1 : NT;
+    float acc[2][AT][4];
 #pragma unroll
     for (int rt = 0; rt < 2; rt++)
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+      for (int t = 0; t < AT; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[rt][t][e] = 0.f;
 
@@ -275,27 +293,28 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
         __syncthreads();  // what was staged before has been read
         const int eights = (end - ch) * 32;
         if (pl.split_x) {
-          constexpr int BYTES = w4_split_bytes(GB), SCALES = 2 * P, SUMS = 2 * GB * P;
+          constexpr int BYTES = w4_split_bytes(GB), FLOATS = 2 + 2 * GB;
           const uint8_t* src = static_cast<const uint8_t*>(a.ws) + (m0 * pairs + ch) * BYTES;
           const int n_pairs = end - ch, words = P * 16;
           for (int i = threadIdx.x; i < mt * n_pairs * words; i += THREADS) {
             const int word = i % words, q = i / words, t = q / n_pairs, pr = q % n_pairs;
-            *reinterpret_cast<uint4*>(xs + (t * P + word / 16) * row_bytes + pr * 256 + word % 16 * 16) =
+            *reinterpret_cast<uint4*>(xs + column(t, word / 16) * row_bytes + pr * 256 + word % 16 * 16) =
                 __ldg(reinterpret_cast<const uint4*>(src + ((int64_t)t * pairs + pr) * BYTES) + word);
           }
-          for (int i = threadIdx.x; i < mt * n_pairs * (SCALES + SUMS); i += THREADS) {
-            const int j = i % (SCALES + SUMS), q = i / (SCALES + SUMS), t = q / n_pairs, pr = q % n_pairs;
-            const int v = __ldg(reinterpret_cast<const int*>(src + ((int64_t)t * pairs + pr) * BYTES + P * 256) + j);
-            if (j < SCALES) xscale[(pr * 2 + j / P) * NT * 8 + t * P + j % P] = __int_as_float(v);
-            else xsum[(pr * 2 * GB + (j - SCALES) / P) * NT * 8 + t * P + (j - SCALES) % P] = v;
+          for (int i = threadIdx.x; i < mt * n_pairs * FLOATS; i += THREADS) {
+            const int j = i % FLOATS, q = i / FLOATS, t = q / n_pairs, pr = q % n_pairs;
+            const float v = __ldg(reinterpret_cast<const float*>(src + ((int64_t)t * pairs + pr) * BYTES + P * 256) + j);
+            if (j < 2) xscale[(pr * 2 + j) * XC + t] = v;
+            else xsum[(pr * 2 * GB + j - 2) * XC + t] = v;
           }
-        } else
-        for (int i = threadIdx.x; i < eights * mt; i += THREADS) {
-          const int t = i / eights, e = i % eights;
-          w4_stage8<GROUP>(a, m0 + t, (int64_t)ch * 256 + e * 8,
-                           xs + t * P * row_bytes + (e >> 4) * 128 + (e & 3) * 32 + ((e >> 2) & 3) * 8,
-                           row_bytes, &xscale[(e >> 4) * NT * 8 + t * P],
-                           &xsum[(e >> 4) * GB * NT * 8 + t * P], NT * 8);
+        } else {
+          for (int i = threadIdx.x; i < eights * mt; i += THREADS) {
+            const int t = i / eights, e = i % eights, at = JOINT ? t : t * P;
+            w4_stage8<GROUP, JOINT>(a, m0 + t, (int64_t)ch * 256 + e * 8,
+                                    xs + column(t, 0) * row_bytes + (e >> 4) * 128 + (e & 3) * 32 + ((e >> 2) & 3) * 8,
+                                    (JOINT ? 8 : 1) * row_bytes, &xscale[(e >> 4) * XC + at],
+                                    &xsum[(e >> 4) * GB * XC + at], XC);
+          }
         }
         __syncthreads();
       }
@@ -316,9 +335,9 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
         const uint8_t* xb[NT];  // column 8 t + n, words 0 and 1
 #pragma unroll
         for (int t = 0; t < NT; t++)
-          xb[t] = (8 * t + n < cols ? xs + (8 * t + n) * row_bytes + (p - ch) * 256 : zeros) + c * 32;
-        const float* bs = xscale + (p - ch) * 2 * NT * 8 + 2 * c;
-        const int* bz = xsum + (p - ch) * 2 * GB * NT * 8 + 2 * c;
+          xb[t] = (has_column(t) ? xs + (8 * t + n) * row_bytes + (p - ch) * 256 : zeros) + c * 32;
+        const float* bs = xscale + (p - ch) * 2 * XC + 2 * c;
+        const float* bz = xsum + (p - ch) * 2 * GB * XC + 2 * c;
         // Two words of one block: 64 inputs of both m16 tiles.
         auto words = [&](int k, int i2, int (&sum)[2][NT][4]) {
           uint4 x[NT];
@@ -355,15 +374,29 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
                   s[r] = w4_scale(m & 0xffffu, sbf);
                   z[r] = (int)(m >> 16);
                 }
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                  const float2 b2 = *reinterpret_cast<const float2*>(bs + k * NT * 8 + 8 * t);
-                  const int2 z2 = *reinterpret_cast<const int2*>(bz + g * NT * 8 + 8 * t);
+                if constexpr (JOINT) {
+                  const float2 b2 = *reinterpret_cast<const float2*>(bs + k * XC);
+                  const float2 z2 = *reinterpret_cast<const float2*>(bz + g * XC);
 #pragma unroll
                   for (int e = 0; e < 4; e++) {
-                    const int v = sum[rt][t][e] - z[e >> 1] * (e & 1 ? z2.y : z2.x);
-                    acc[rt][t][e] = fmaf(__int_as_float(v) - 12582912.f, s[e >> 1] * (e & 1 ? b2.y : b2.x),
-                                         acc[rt][t][e]);
+                    float v[3];
+#pragma unroll
+                    for (int q = 0; q < 3; q++) v[q] = __int_as_float(sum[rt][q][e]) - 12582912.f;
+                    const float whole = fmaf(v[0], 65536.f, fmaf(v[1], 256.f, v[2]));
+                    acc[rt][0][e] = fmaf(fmaf(-(float)z[e >> 1], e & 1 ? z2.y : z2.x, whole),
+                                         s[e >> 1] * (e & 1 ? b2.y : b2.x), acc[rt][0][e]);
+                  }
+                } else {
+#pragma unroll
+                  for (int t = 0; t < NT; t++) {
+                    const float2 b2 = *reinterpret_cast<const float2*>(bs + k * XC + 8 * t);
+                    const int2 z2 = *reinterpret_cast<const int2*>(bz + g * XC + 8 * t);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                      const int v = sum[rt][t][e] - z[e >> 1] * (e & 1 ? z2.y : z2.x);
+                      acc[rt][t][e] = fmaf(__int_as_float(v) - 12582912.f, s[e >> 1] * (e & 1 ? b2.y : b2.x),
+                                           acc[rt][t][e]);
+                    }
                   }
                 }
               }
@@ -398,7 +431,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
     for (int rt = 0; rt < 2; rt++) {
       __syncthreads();  // the sums before have been read
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+      for (int t = 0; t < AT; t++)
 #pragma unroll
         for (int h = 0; h < 2; h++)
           *reinterpret_cast<float2*>(&red[(warp * 16 + h * 8 + n) * LD + t * 8 + 2 * c]) =
@@ -409,8 +442,8 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
         const int r = i % rows, t = i / rows, w = r / 16, rr = r % 16;
         float v = 0.f;
         for (int k = 0; k < pl.wk; k++) {
-          const float* s = red + ((w * pl.wk + k) * 16 + rr) * LD + t * P;
-          v += (s[2] + s[1]) + s[0];
+          const float* s = red + ((w * pl.wk + k) * 16 + rr) * LD + (JOINT ? t : t * P);
+          v += JOINT ? s[0] : (s[2] + s[1]) + s[0];
         }
         const int row = w * kW4Tile + rt * 16 + rr;
         if (pl.split > 1) part[(buf * pl.mt + t) * cta_rows + row] = v;
@@ -443,7 +476,9 @@ static int w4_pass_rows(int64_t m) {
   const int64_t passes = (m + kW4Rows - 1) / kW4Rows;
   return (int)((m + passes - 1) / passes);
 }
-static int w4_column_tiles(int64_t m) { return (w4_pass_rows(m) * kW4Planes + 7) / 8; }
+static int w4_column_tiles(int64_t m) {
+  return m > kW4Rows ? 3 : (int)(m * kW4Planes + 7) / 8;
+}
 
 size_t linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t) {
   if (m <= kW4Rows) return 0;
@@ -464,8 +499,8 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
   const int64_t passes = (m + kW4Rows - 1) / kW4Rows;
   p.mt = w4_pass_rows(m);
   p.split_x = m > kW4Rows;
-  const int cols = p.mt * kW4Planes;
   p.nt = w4_column_tiles(m);
+  const int cols = p.nt == 3 ? 24 : p.mt * kW4Planes, xc = p.nt == 3 ? 8 : 8 * p.nt;
   const int64_t tiles = (out_f + kW4Tile - 1) / kW4Tile, pairs = (in_f + 255) / 256;
   const int warps = w4_warps(p.nt);
   const int fixed = w4_ring_bytes(p.nt) + w4_red_bytes(p.nt);
@@ -476,7 +511,7 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
       const int part = split > 1 ? 2 * p.mt * wr * kW4Tile * 4 : 0;
       const int64_t range = (pairs + split - 1) / split;
       const int64_t left = w4_smem(p.nt) - fixed - part - 16 * cols - 256;
-      const int64_t fit = std::max<int64_t>(left, 0) / (256 * cols + 64 * p.nt * (1 + gb)) / wk * wk;
+      const int64_t fit = std::max<int64_t>(left, 0) / (256 * cols + 8 * xc * (1 + gb)) / wk * wk;
       if (fit == 0) continue;  // chunks are whole turns of the wk warps
       const int64_t chunk = std::min(range, fit);
       const int64_t units = (tiles + wr - 1) / wr;
@@ -502,7 +537,7 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
         p.chunk = (int)chunk;
         p.units = (int)units;
         p.grid = (int)grid;
-        p.smem = fixed + part + (int)chunk * 64 * p.nt * (1 + gb) + 256 + cols * (int)(chunk * 256 + 16);
+        p.smem = fixed + part + (int)chunk * 8 * xc * (1 + gb) + 256 + cols * (int)(chunk * 256 + 16);
       }
     }
   return p;
