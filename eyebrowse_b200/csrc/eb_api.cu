@@ -1067,7 +1067,12 @@ int eb_attention_decode_kv8(const eb_attn_desc* d, const eb_attn_layer* L, const
                    (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return EB_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (k) {
+  // The tensor-core kernel appends by itself where one CTA has all query heads
+  // of a KV head; elsewhere the write is a launch of its own in front.
+  const bool tc = kv8_tc_supported(d->head_dim);
+  const Kv8Plan p = tc ? plan_kv8(d, batch, max_pos) : Kv8Plan{};
+  const bool fused = tc && p.gsubs == 1;
+  if (k && !fused) {
     Kv8WriteArgs w = kv8_write_args(d, L, c, k, v);
     w.start = max_pos;
     w.count = 1;
@@ -1105,8 +1110,15 @@ int eb_attention_decode_kv8(const eb_attn_desc* d, const eb_attn_layer* L, const
   a.sin_t = L ? L->rope_sin : nullptr;
   a.eps = d->eps;
   a.scale_log2 = d->scale * kLog2e;
-  if (!kv8_tc_supported(d->head_dim)) return cuda_status(launch_kv8_decode(a, st));
-  const Kv8Plan p = plan_kv8(d, batch, max_pos);
+  if (!tc) return cuda_status(launch_kv8_decode(a, st));
+  if (k && fused) {
+    a.k_new = k;
+    a.v_new = v;
+    a.kv_bstride = kvs_of(d);
+    a.kv_aligned = aligned16(k) && aligned16(v) && ((kvs_of(d) * elem_bytes(d->dtype_qkv)) & 15) == 0;
+    a.k_norm_w = L ? L->k_norm_w : nullptr;
+    a.v_norm_w = L ? L->v_norm_w : nullptr;
+  }
   const DecodePlan w = kv8_layout(d, batch, p.cmax);
   a.gsubs = p.gsubs;
   a.chunk = p.chunk;

@@ -210,6 +210,14 @@ struct Kv8DecodeArgs {
   const float* cos_t;
   const float* sin_t;
   float eps, scale_log2;
+  // the new rows that the tensor-core kernel appends itself (k_new null: none);
+  // they have dtype_q
+  const void* k_new;
+  const void* v_new;
+  int64_t kv_bstride;
+  bool kv_aligned;  // may be read in 16-byte words
+  const float* k_norm_w;
+  const float* v_norm_w;
   // tensor-core kernel: head groups per KV head, rows per chunk (a multiple of
   // 128), chunks of the longest context, split-K workspace
   int gsubs, chunk, cmax;

@@ -20,55 +20,6 @@ namespace eb {
 // first is used, so every byte is read once and written once. It is bound by
 // HBM: 8192 rows of 8 heads of 128 in bf16 (50 MB) take KV8_WRITE_US us.
 // kv8_write_kernel (any other head_dim) stages them as f32 in shared memory.
-template <int E, bool E5M2>
-__device__ __forceinline__ void f8_store(uint8_t* p, const float (&v)[E], float inv) {
-  uint32_t w[(E + 3) / 4] = {};
-#pragma unroll
-  for (int e = 0; e < E; e += 2)
-    w[e / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[e] * inv, v[e + 1] * inv),
-                                                   __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3)
-                << (8 * (e & 3));
-  if constexpr (E == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
-  else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-  else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-}
-
-// E neighbouring elements: one or two loads where `aligned`, as they lie.
-template <typename T, int E>
-struct RawRow {
-  static constexpr int W = E * (int)sizeof(T) / 4;
-  uint32_t w[W];
-  __device__ __forceinline__ void load(const T* p, bool aligned) {
-    if (aligned) {
-      if constexpr (W == 1) {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-      } else if constexpr (W == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x;
-        w[1] = u.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < W; i += 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
-          w[i] = u.x;
-          w[i + 1] = u.y;
-          w[i + 2] = u.z;
-          w[i + 3] = u.w;
-        }
-      }
-    } else {
-      T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-      for (int i = 0; i < E; i++) e[i] = p[i];
-    }
-  }
-  __device__ __forceinline__ void f32(float (&f)[E]) const {
-    const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < E; i++) f[i] = Elem<T>::to_f32(e[i]);
-  }
-};
-
 // CTAs of the same rows (K and V, every head) are neighbours: together they
 // read and write whole rows.
 template <typename T, int E, int R>

@@ -25,8 +25,9 @@
 // One CTA = (KV head [, 8 of its heads], sequence, chunk of rows), 192
 // threads: warps 0-3 softmax and output, warp 4 TMA producer, warp 5 TMEM owner
 // and MMA issuer (S of tile j + 1 runs during the softmax of tile j). Chunks
-// start on multiples of 128 rows, so a block of rows never spans two. The last
-// CTA of a (sequence, head group) merges the chunks' partial (m, l, O) in chunk
+// start on multiples of 128 rows, so a block of rows never spans two; the CTA of
+// the last one appends the step's new row first (two warps each for K and V),
+// where one CTA has all heads of the KV head. The last CTA of a (sequence, head group) merges the chunks' partial (m, l, O) in chunk
 // order (atomic ticket, no spin-wait).
 #include "eb_kv8.cuh"
 #include "eb_rowops.cuh"
@@ -124,6 +125,7 @@ __global__ void __launch_bounds__(192)
   const int row_begin = first + ck * a.chunk;
   const int row_end = min(row_begin + a.chunk, pos + 1);
   const int n_tiles = (row_end - row_begin + kKvTile - 1) / kKvTile;
+  const bool append = a.k_new && ck == n_chunks - 1;  // this chunk holds the new row and its block
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(192)
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   constexpr int kQ = 0, kFinal = 1, kSFull0 = 2, kPFull0 = 4, kODone0 = 6, kKFull0 = 8;
   constexpr int kKEmpty0 = kKFull0 + NST, kVFull0 = kKEmpty0 + NST, kVEmpty0 = kVFull0 + NST;
-  constexpr int kNumBars = kVEmpty0 + NST;
+  constexpr int kAppended = kVEmpty0 + NST, kNumBars = kAppended + 1;
   static_assert(kNumBars * 8 <= 256, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(192)
     mbar_init(bar(kQ), 128);
     mbar_init(bar(kFinal), 1);
     for (int i = kSFull0; i < kNumBars; i++)
-      mbar_init(bar(i), i == kPFull0 || i == kPFull0 + 1 ? 128 : 1);
+      mbar_init(bar(i), i == kPFull0 || i == kPFull0 + 1 || i == kAppended ? 128 : 1);
     *abort_flag = 0;
     fence_mbar_init();
     fence_async_smem();
@@ -168,7 +170,8 @@ __global__ void __launch_bounds__(192)
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int issued = 0;
-      bool ok = true;
+      // only the chunk that is appended to waits for it
+      bool ok = !append || mbar_wait(bar(kAppended), 0, abort_flag, a.err, kErrTimeoutTma);
       for (int j = 0; ok && j < n_tiles; j++) {
         const int st = j % NST, row = row_begin + j * kKvTile;
         for (int which = 0; which < 2; which++) {
@@ -249,6 +252,12 @@ __global__ void __launch_bounds__(192)
   } else {
     // ------------------------------------------------------------ softmax (warps 0-3)
     const int tid = threadIdx.x;
+    if (append) {  // warps 0 and 1 the K row, 2 and 3 the V row
+      kv8_append<E>(a, warp >> 1, b, kvh, pos, warp & 1, lane, 2 + (warp >> 1));
+      // generic-proxy writes -> visible to the TMA loads that follow
+      asm volatile("fence.proxy.async.global;" ::: "memory");
+      mbar_arrive(bar(kAppended));
+    }
     // Q's planes: a warp per head, a head's largest value brought to [128, 256)
     float* qscale = wsum;  // [8] until the sums need the place
     for (int g = warp; g < G; g += 4) {
@@ -296,8 +305,9 @@ __global__ void __launch_bounds__(192)
     auto scales = [&](int j, float& k, float& v) {  // of this thread's row of tile j
       const int row = row_begin + j * kKvTile + tid;
       const bool in = row >= row_lo && row < row_end;
-      k = in ? __ldg(ks + (int64_t)(row >> shift) * a.hkv) : 0.f;
-      v = in ? __ldg(vs + (int64_t)(row >> shift) * a.hkv) : 0.f;
+      // (through L2: the append wrote one of them)
+      k = in ? __ldcg(ks + (int64_t)(row >> shift) * a.hkv) : 0.f;
+      v = in ? __ldcg(vs + (int64_t)(row >> shift) * a.hkv) : 0.f;
     };
     float m[GP], l[GP];
 #pragma unroll
