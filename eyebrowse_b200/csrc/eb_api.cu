@@ -1007,7 +1007,7 @@ int eb_kv8_write(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
 
 // Split of the contexts of an 8-bit decode call into chunks of whole 128-row
 // tiles: about as many CTAs as the SMs hold at once (two each at head_dim 128,
-// one at 256), chunks of at most 64 tiles so that unequal contexts even out,
+// one at 256), chunks of at most 32 tiles so that unequal contexts even out,
 // at most 256 of them.
 struct Kv8Plan {
   int gsubs, chunk, cmax;
@@ -1021,12 +1021,12 @@ static Kv8Plan plan_kv8(const eb_attn_desc* d, int64_t batch, int64_t max_pos) {
       max_pos / 128 + 1, d->window > 0 ? ((int64_t)d->window + 126) / 128 + 1 : INT64_MAX);
   const int64_t n = batch * d->n_kv_heads * p.gsubs;
   const int64_t target = (d->head_dim == 128 ? 2 : 1) * (int64_t)sm_count();
-  int64_t c = std::min<int64_t>((tiles * n + target - 1) / target, 64);
+  int64_t c = std::min<int64_t>((tiles * n + target - 1) / target, 32);
   c = std::max<int64_t>(c, (tiles + 255) / 256);
   p.chunk = (int)c * 128;
   p.cmax = (int)((tiles + c - 1) / c);
   p.bound = std::min(std::min<int64_t>(tiles, 256),
-                     std::max((target + n - 1) / n, (tiles + 63) / 64));
+                     std::max((target + n - 1) / n, (tiles + 31) / 32));
   return p;
 }
 static DecodePlan kv8_layout(const eb_attn_desc* d, int64_t batch, int64_t chunks) {

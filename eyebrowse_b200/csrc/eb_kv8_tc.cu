@@ -105,6 +105,20 @@ __device__ __forceinline__ void f8_planes(float x, uint8_t (&c)[P]) {
   }
 }
 
+// The same of two values: codes of x0 in the low, of x1 in the high byte.
+template <int P>
+__device__ __forceinline__ void f8_planes2(float x0, float x1, uint16_t (&c)[P]) {
+#pragma unroll
+  for (int j = 0; j < P; j++) {
+    c[j] = __nv_cvt_float2_to_fp8x2(make_float2(x0, x1), __NV_SATFINITE, __NV_E4M3);
+    if (j + 1 < P) {
+      const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c[j], __NV_E4M3)));
+      x0 = (x0 - v.x) * 16.f;
+      x1 = (x1 - v.y) * 16.f;
+    }
+  }
+}
+
 template <int HD, int GP, int P>
 __global__ void __launch_bounds__(192)
     kv8_decode_tc_kernel(const __grid_constant__ CUtensorMap tmK,
@@ -339,19 +353,27 @@ __global__ void __launch_bounds__(192)
 #pragma unroll
         for (int p = P - 2; p >= 0; p--) x = fmaf(x, 0.0625f, __uint_as_float(raw[h * P + p]));
         s[h] = in ? x * (qs[h] * ksc) : -INFINITY;
-        const float top = warp_max(s[h] + lv);
-        if (lane == 0 && h < G) wmax[(buf * 4 + warp) * 8 + h] = top;
       }
-      ok = named_bar_and(1, 128, ok);
-      if (!ok) break;
-      float mn[GP];
-      bool raise = false;
+      // Does a row pass the reference of its head by too much? One barrier tells
+      // all four warps; only then are the tile's maxima exchanged.
+      bool over = false;
 #pragma unroll
-      for (int h = 0; h < GP; h++) {
-        if (h >= G) continue;
-        const float* w = wmax + buf * 32 + h;
-        mn[h] = fmaxf(fmaxf(w[0], w[8]), fmaxf(w[16], w[24]));
-        raise = raise || mn[h] > m[h] + kKvRescale;
+      for (int h = 0; h < GP; h++) over = over || (h < G && s[h] + lv > m[h] + kKvRescale);
+      bool raise = !named_bar_and(1, 128, ok && !over);
+      float mn[GP];
+      if (raise) {
+#pragma unroll
+        for (int h = 0; h < GP; h++) {
+          const float top = warp_max(s[h] + lv);
+          if (lane == 0 && h < G) wmax[(buf * 4 + warp) * 8 + h] = top;
+        }
+        ok = named_bar_and(1, 128, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < GP; h++) {
+          const float* w = wmax + buf * 32 + h;
+          mn[h] = h < G ? fmaxf(fmaxf(w[0], w[8]), fmaxf(w[16], w[24])) : 0.f;
+        }
       }
       if (raise) {  // the same in all four warps
         float corr[GP];
@@ -390,15 +412,29 @@ __global__ void __launch_bounds__(192)
       if (j >= 2)
         ok = ok && mbar_wait(bar(kODone0 + buf), ((j >> 1) - 1) & 1, abort_flag, a.err, kErrTimeoutSoftmax);
       uint8_t* pt = smem + C::P_OFF + buf * C::ROWS;
+      const float vp = in ? vsc * kPScale : 0.f;
 #pragma unroll
-      for (int h = 0; h < GP; h++) {
+      for (int h = 0; h < GP; h += 2) {
         if (h >= G) continue;
-        const float w = in ? ex2(s[h] - m[h]) : 0.f;
-        l[h] += w;
-        uint8_t c[P];
-        f8_planes<P>(in ? w * (vsc * kPScale) : 0.f, c);
+        // (a head past G has a score of garbage: its columns are not read)
+        const float w0 = in ? ex2(s[h] - m[h]) : 0.f;
+        l[h] += w0;
+        if constexpr (GP == 1) {
+          uint8_t c[P];
+          f8_planes<P>(in ? w0 * vp : 0.f, c);
 #pragma unroll
-        for (int p = 0; p < P; p++) pt[sw128_byte(h * P + p, tid)] = c[p];
+          for (int p = 0; p < P; p++) pt[sw128_byte(p, tid)] = c[p];
+        } else {
+          const float w1 = in ? ex2(s[h + 1] - m[h + 1]) : 0.f;
+          l[h + 1] += w1;
+          uint16_t c[P];
+          f8_planes2<P>(in ? w0 * vp : 0.f, in ? w1 * vp : 0.f, c);
+#pragma unroll
+          for (int p = 0; p < P; p++) {
+            pt[sw128_byte(h * P + p, tid)] = (uint8_t)c[p];
+            pt[sw128_byte((h + 1) * P + p, tid)] = (uint8_t)(c[p] >> 8);
+          }
+        }
       }
       if (row_begin + j * kKvTile < row_lo || row_begin + (j + 1) * kKvTile > row_end) {
         // Rows outside [row_lo, row_end) hold whatever the cache holds, NaN
