@@ -1006,8 +1006,8 @@ int eb_kv8_write(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8* c,
 }
 
 // Split of the contexts of an 8-bit decode call into chunks of whole 128-row
-// tiles: about as many CTAs as the SMs hold at once (two each at head_dim 128,
-// one at 256), chunks of at most 32 tiles so that unequal contexts even out,
+// tiles: about as many CTAs as the SMs hold at once (one each at head_dim 256,
+// else two), chunks of at most 32 tiles so that unequal contexts even out,
 // at most 256 of them.
 struct Kv8Plan {
   int gsubs, chunk, cmax;
@@ -1015,12 +1015,14 @@ struct Kv8Plan {
 };
 static Kv8Plan plan_kv8(const eb_attn_desc* d, int64_t batch, int64_t max_pos) {
   Kv8Plan p{};
-  p.gsubs = (d->n_heads / d->n_kv_heads + 7) / 8;
+  // a CTA has 8 heads of a KV head; at head_dim 64 4 of each of two
+  const bool pair = d->head_dim == 64;
+  p.gsubs = (d->n_heads / d->n_kv_heads + (pair ? 3 : 7)) / (pair ? 4 : 8);
   // a window may begin inside a tile
   const int64_t tiles = std::min<int64_t>(
       max_pos / 128 + 1, d->window > 0 ? ((int64_t)d->window + 126) / 128 + 1 : INT64_MAX);
-  const int64_t n = batch * d->n_kv_heads * p.gsubs;
-  const int64_t target = (d->head_dim == 128 ? 2 : 1) * (int64_t)sm_count();
+  const int64_t n = batch * (pair ? (d->n_kv_heads + 1) / 2 : d->n_kv_heads) * p.gsubs;
+  const int64_t target = (d->head_dim == 256 ? 1 : 2) * (int64_t)sm_count();
   int64_t c = std::min<int64_t>((tiles * n + target - 1) / target, 32);
   c = std::max<int64_t>(c, (tiles + 255) / 256);
   p.chunk = (int)c * 128;

@@ -1,5 +1,5 @@
 // eb_kv8_tc.cu -- decode attention over the 8-bit cache on tcgen05 tensor cores
-// (head_dim 128 and 256).
+// (head_dim 64, 128 and 256).
 //
 // The cache's bytes go from HBM through TMA into shared memory and from there
 // into the tensor core as they are: no thread touches them. For a KV head and
@@ -16,13 +16,18 @@
 // G * planes columns are few, so the tensor work stays far below the time the
 // bytes take (N = 48: two MMAs of 24 clocks per 4 KB).
 //
+// At head_dim 64 a CTA takes two neighbouring KV heads, whose bytes of a row lie
+// side by side: their tile looks like one of head_dim 128. S is made for each
+// from its own half of the bytes; O for the heads of both, of which each keeps
+// its own half of the lanes.
+//
 // Scales: a row's K scale multiplies its scores, its V scale its weight, both
 // in the softmax thread that owns the row (one TMEM lane each). Weights are
 // kept relative to a running maximum of score + log2(V scale) per head, so
 // that what P holds stays in E4M3's range; it is raised (and O rescaled) only
 // when a tile passes it by more than 2^3.5.
 //
-// One CTA = (KV head [, 8 of its heads], sequence, chunk of rows), 192
+// One CTA = (KV head or pair [, 8 heads of it], sequence, chunk of rows), 192
 // threads: warps 0-3 softmax and output, warp 4 TMA producer, warp 5 TMEM owner
 // and MMA issuer (S of tile j + 1 runs during the softmax of tile j). Chunks
 // start on multiples of 128 rows, so a block of rows never spans two; the CTA of
@@ -42,8 +47,12 @@ constexpr float kMinLogScale = -64.f;  // of a V scale of zero
 
 template <int HD, int GP, int P>
 struct Kv8Cfg {
-  static constexpr int HB = HD / 128;
-  static constexpr int N = (GP * P + 15) / 16 * 16;
+  static constexpr bool PAIR = HD == 64;  // two KV heads, GP / 2 query heads of each
+  static constexpr int HALVES = PAIR ? 2 : 1, GH = GP / HALVES;
+  static constexpr int HB = PAIR ? 1 : HD / 128;
+  static constexpr int NH = (GH * P + 15) / 16 * 16, N = HALVES * NH;  // columns of a KV head, of a tile
+  // column of plane p of head h
+  static constexpr __host__ __device__ int col(int h, int p) { return h / GH * NH + h % GH * P + p; }
   static constexpr int ROWS = N * 128;  // bytes of a [N][128] operand block
   static constexpr int TILE = kKvTile * 128;
   static constexpr int K_BYTES = HB * TILE;
@@ -124,12 +133,14 @@ __global__ void __launch_bounds__(192)
     kv8_decode_tc_kernel(const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, Kv8DecodeArgs a) {
   using C = Kv8Cfg<HD, GP, P>;
-  constexpr int E = HD / 32, N = C::N, NST = C::NST;
+  constexpr int E = HD / 32, N = C::N, NST = C::NST, GH = C::GH, HALVES = C::HALVES;
   const int grp = blockIdx.x, b = blockIdx.y, ck = blockIdx.z;
-  const int kvh = grp / a.gsubs, sub = grp % a.gsubs;
+  const int kvh = grp / a.gsubs * HALVES, sub = grp % a.gsubs;
   const int heads = a.H / a.hkv;
-  const int head0 = kvh * heads + sub * GP;
-  const int G = min(GP, heads - sub * GP);
+  const int G = min(GH, heads - sub * GH);           // heads of each KV head
+  const int halves = min(HALVES, a.hkv - kvh);       // an odd last KV head has no neighbour
+  auto has = [&](int h) { return h % GH < G && h / GH < halves; };
+  auto head = [&](int h) { return (kvh + h / GH) * heads + sub * GH + h % GH; };
   const int pos = a.positions ? a.positions[b] : a.max_pos;
   if (pos < 0 || pos > a.max_pos) return;  // an empty slot of the batch
   const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
@@ -199,7 +210,8 @@ __global__ void __launch_bounds__(192)
           mbar_arrive_expect_tx(bar(full), C::K_BYTES);
 #pragma unroll
           for (int hb = 0; hb < C::HB; hb++)
-            tma_load_4d(dst + hb * C::TILE, which ? &tmV : &tmK, bar(full), hb * 128, kvh, row, b);
+            tma_load_4d(dst + hb * C::TILE, which ? &tmV : &tmK, bar(full),
+                        C::PAIR ? kvh * HD : hb * 128, C::PAIR ? 0 : kvh, row, b);
           issued++;
         }
       }
@@ -216,13 +228,18 @@ __global__ void __launch_bounds__(192)
   } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      const uint32_t id_qk = idesc_f8(N, a.e5m2, false), id_pv = idesc_f8(N, a.e5m2, true);
+      const uint32_t id_qk = idesc_f8(C::NH, a.e5m2, false), id_pv = idesc_f8(N, a.e5m2, true);
       auto issue_qk = [&](int buf, int st) {
 #pragma unroll
-        for (int k = 0; k < HD / 32; k++)
-          umma_f8(tmem + C::S_COL + buf * N,
-                  sdesc_sw128(sKV + st * 2 * C::K_BYTES + (k >> 2) * C::TILE + (k & 3) * 32, 16, 1024),
-                  sdesc_sw128(sQ + (k >> 2) * C::ROWS + (k & 3) * 32, 16, 1024), id_qk, k > 0);
+        for (int u = 0; u < HALVES; u++)  // (a pair's second KV head: bytes 64.. of the rows)
+#pragma unroll
+          for (int k = 0; k < HD / 32; k++) {
+            const int at = u * 2 + k;
+            umma_f8(tmem + C::S_COL + buf * N + u * C::NH,
+                    sdesc_sw128(sKV + st * 2 * C::K_BYTES + (at >> 2) * C::TILE + (at & 3) * 32, 16, 1024),
+                    sdesc_sw128(sQ + (at >> 2) * C::ROWS + u * C::NH * 128 + (at & 3) * 32, 16, 1024),
+                    id_qk, k > 0);
+          }
       };
       auto issue_pv = [&](int buf, int st, bool first_tile) {
 #pragma unroll
@@ -267,16 +284,18 @@ __global__ void __launch_bounds__(192)
     // ------------------------------------------------------------ softmax (warps 0-3)
     const int tid = threadIdx.x;
     if (append) {  // warps 0 and 1 the K row, 2 and 3 the V row
-      kv8_append<E>(a, warp >> 1, b, kvh, pos, warp & 1, lane, 2 + (warp >> 1));
+      for (int u = 0; u < halves; u++)
+        kv8_append<E>(a, warp >> 1, b, kvh + u, pos, warp & 1, lane, 2 + (warp >> 1));
       // generic-proxy writes -> visible to the TMA loads that follow
       asm volatile("fence.proxy.async.global;" ::: "memory");
       mbar_arrive(bar(kAppended));
     }
     // Q's planes: a warp per head, a head's largest value brought to [128, 256)
     float* qscale = wsum;  // [8] until the sums need the place
-    for (int g = warp; g < G; g += 4) {
+    for (int g = warp; g < GP; g += 4) {
+      if (!has(g)) continue;
       float v[E];
-      const int64_t at = (int64_t)b * a.q_bstride + (int64_t)(head0 + g) * HD + lane * E;
+      const int64_t at = (int64_t)b * a.q_bstride + (int64_t)head(g) * HD + lane * E;
       if (((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_bstride * (a.dtype_q == kF32 ? 4 : 2))) & 15) == 0) {
         ld_row<E>(a.q, at, a.dtype_q, v);
       } else {
@@ -296,14 +315,18 @@ __global__ void __launch_bounds__(192)
 #pragma unroll
       for (int e = 0; e < E; e++)
         f8_planes<P>(fabsf(v[e]) <= 3.402823466e38f ? v[e] * up : __uint_as_float(0x7fc00000u), c[e]);
-      const int d = lane * E;
+      const int d = g / GH * 64 + lane * E;
 #pragma unroll
       for (int j = 0; j < P; j++) {
-        uint8_t* dst = smem + C::Q_OFF + (d >> 7) * C::ROWS + sw128_byte(g * P + j, d & 127);
+        uint8_t* dst = smem + C::Q_OFF + (d >> 7) * C::ROWS + sw128_byte(C::col(g, j), d & 127);
+        if constexpr (E == 2) {
+          *reinterpret_cast<uint16_t*>(dst) = (uint16_t)(c[0][j] | c[1][j] << 8);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<uint32_t*>(dst + e) = (uint32_t)c[e][j] | (uint32_t)c[e + 1][j] << 8 |
-                                                  (uint32_t)c[e + 2][j] << 16 | (uint32_t)c[e + 3][j] << 24;
+          for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<uint32_t*>(dst + e) = (uint32_t)c[e][j] | (uint32_t)c[e + 1][j] << 8 |
+                                                    (uint32_t)c[e + 2][j] << 16 | (uint32_t)c[e + 3][j] << 24;
+        }
       }
     }
     fence_async_smem();
@@ -311,17 +334,19 @@ __global__ void __launch_bounds__(192)
     named_bar_and(1, 128, true);
     float qs[GP];
 #pragma unroll
-    for (int h = 0; h < GP; h++) qs[h] = h < G ? qscale[h] * a.scale_log2 : 0.f;
+    for (int h = 0; h < GP; h++) qs[h] = has(h) ? qscale[h] * a.scale_log2 : 0.f;
 
     const float* ks = a.k_scale + b * a.scale_bstride + kvh;
     const float* vs = a.v_scale + b * a.scale_bstride + kvh;
     const int shift = 31 - __clz(a.block);
-    auto scales = [&](int j, float& k, float& v) {  // of this thread's row of tile j
+    auto scales = [&](int j, float (&k)[HALVES], float (&v)[HALVES]) {  // of this thread's row of tile j
       const int row = row_begin + j * kKvTile + tid;
       const bool in = row >= row_lo && row < row_end;
-      // (through L2: the append wrote one of them)
-      k = in ? __ldcg(ks + (int64_t)(row >> shift) * a.hkv) : 0.f;
-      v = in ? __ldcg(vs + (int64_t)(row >> shift) * a.hkv) : 0.f;
+#pragma unroll
+      for (int u = 0; u < HALVES; u++) {  // (through L2: the append wrote one of them)
+        k[u] = in && u < halves ? __ldcg(ks + (int64_t)(row >> shift) * a.hkv + u) : 0.f;
+        v[u] = in && u < halves ? __ldcg(vs + (int64_t)(row >> shift) * a.hkv + u) : 0.f;
+      }
     };
     float m[GP], l[GP];
 #pragma unroll
@@ -329,7 +354,7 @@ __global__ void __launch_bounds__(192)
       m[h] = -INFINITY;
       l[h] = 0.f;
     }
-    float ksc, vsc, ksn = 0.f, vsn = 0.f;
+    float ksc[HALVES], vsc[HALVES], ksn[HALVES] = {}, vsn[HALVES] = {};
     scales(0, ksc, vsc);
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     bool ok = true;
@@ -345,34 +370,39 @@ __global__ void __launch_bounds__(192)
       tmem_ld_wait();
       const int row = row_begin + j * kKvTile + tid;
       const bool in = row >= row_lo && row < row_end;
-      const float lv = vsc > 0x1p-64f ? __log2f(vsc) : kMinLogScale;
+      float lv[HALVES], vp[HALVES];
+#pragma unroll
+      for (int u = 0; u < HALVES; u++) {
+        lv[u] = vsc[u] > 0x1p-64f ? __log2f(vsc[u]) : kMinLogScale;
+        vp[u] = in ? vsc[u] * kPScale : 0.f;
+      }
       float s[GP];
 #pragma unroll
       for (int h = 0; h < GP; h++) {
-        float x = __uint_as_float(raw[h * P + P - 1]);
+        float x = __uint_as_float(raw[C::col(h, P - 1)]);
 #pragma unroll
-        for (int p = P - 2; p >= 0; p--) x = fmaf(x, 0.0625f, __uint_as_float(raw[h * P + p]));
-        s[h] = in ? x * (qs[h] * ksc) : -INFINITY;
+        for (int p = P - 2; p >= 0; p--) x = fmaf(x, 0.0625f, __uint_as_float(raw[C::col(h, p)]));
+        s[h] = in ? x * (qs[h] * ksc[h / GH]) : -INFINITY;
       }
       // Does a row pass the reference of its head by too much? One barrier tells
       // all four warps; only then are the tile's maxima exchanged.
       bool over = false;
 #pragma unroll
-      for (int h = 0; h < GP; h++) over = over || (h < G && s[h] + lv > m[h] + kKvRescale);
+      for (int h = 0; h < GP; h++) over = over || (has(h) && s[h] + lv[h / GH] > m[h] + kKvRescale);
       bool raise = !named_bar_and(1, 128, ok && !over);
       float mn[GP];
       if (raise) {
 #pragma unroll
         for (int h = 0; h < GP; h++) {
-          const float top = warp_max(s[h] + lv);
-          if (lane == 0 && h < G) wmax[(buf * 4 + warp) * 8 + h] = top;
+          const float top = warp_max(s[h] + lv[h / GH]);
+          if (lane == 0 && has(h)) wmax[(buf * 4 + warp) * 8 + h] = top;
         }
         ok = named_bar_and(1, 128, ok);
         if (!ok) break;
 #pragma unroll
         for (int h = 0; h < GP; h++) {
           const float* w = wmax + buf * 32 + h;
-          mn[h] = h < G ? fmaxf(fmaxf(w[0], w[8]), fmaxf(w[16], w[24])) : 0.f;
+          mn[h] = has(h) ? fmaxf(fmaxf(w[0], w[8]), fmaxf(w[16], w[24])) : 0.f;
         }
       }
       if (raise) {  // the same in all four warps
@@ -380,7 +410,7 @@ __global__ void __launch_bounds__(192)
 #pragma unroll
         for (int h = 0; h < GP; h++) {
           corr[h] = 1.f;
-          if (h >= G) continue;
+          if (!has(h)) continue;
           const float up = fmaxf(m[h], mn[h]);
           corr[h] = m[h] == up ? 1.f : ex2(m[h] - up);
           m[h] = up;
@@ -401,7 +431,7 @@ __global__ void __launch_bounds__(192)
             for (int h = 0; h < GP; h++)
 #pragma unroll
               for (int p = 0; p < P; p++)
-                o[h * P + p] = __float_as_uint(__uint_as_float(o[h * P + p]) * corr[h]);
+                o[C::col(h, p)] = __float_as_uint(__uint_as_float(o[C::col(h, p)]) * corr[h]);
 #pragma unroll
             for (int i = 0; i < N; i += 16) tmem_st16(tmem + lanes + C::O_COL + hb * N + i, o + i);
           }
@@ -412,27 +442,26 @@ __global__ void __launch_bounds__(192)
       if (j >= 2)
         ok = ok && mbar_wait(bar(kODone0 + buf), ((j >> 1) - 1) & 1, abort_flag, a.err, kErrTimeoutSoftmax);
       uint8_t* pt = smem + C::P_OFF + buf * C::ROWS;
-      const float vp = in ? vsc * kPScale : 0.f;
 #pragma unroll
       for (int h = 0; h < GP; h += 2) {
-        if (h >= G) continue;
-        // (a head past G has a score of garbage: its columns are not read)
+        if (!has(h)) continue;
+        // (a head past the last has a score of garbage: its columns are not read)
         const float w0 = in ? ex2(s[h] - m[h]) : 0.f;
         l[h] += w0;
         if constexpr (GP == 1) {
           uint8_t c[P];
-          f8_planes<P>(in ? w0 * vp : 0.f, c);
+          f8_planes<P>(in ? w0 * vp[0] : 0.f, c);
 #pragma unroll
           for (int p = 0; p < P; p++) pt[sw128_byte(p, tid)] = c[p];
         } else {
           const float w1 = in ? ex2(s[h + 1] - m[h + 1]) : 0.f;
           l[h + 1] += w1;
           uint16_t c[P];
-          f8_planes2<P>(in ? w0 * vp : 0.f, in ? w1 * vp : 0.f, c);
+          f8_planes2<P>(in ? w0 * vp[h / GH] : 0.f, in ? w1 * vp[(h + 1) / GH] : 0.f, c);
 #pragma unroll
           for (int p = 0; p < P; p++) {
-            pt[sw128_byte(h * P + p, tid)] = (uint8_t)c[p];
-            pt[sw128_byte((h + 1) * P + p, tid)] = (uint8_t)(c[p] >> 8);
+            pt[sw128_byte(C::col(h, p), tid)] = (uint8_t)c[p];
+            pt[sw128_byte(C::col(h + 1, p), tid)] = (uint8_t)(c[p] >> 8);
           }
         }
       }
@@ -452,8 +481,11 @@ __global__ void __launch_bounds__(192)
       fence_async_smem();
       tc_fence_before();
       mbar_arrive(bar(kPFull0 + buf));
-      ksc = ksn;
-      vsc = vsn;
+#pragma unroll
+      for (int u = 0; u < HALVES; u++) {
+        ksc[u] = ksn[u];
+        vsc[u] = vsn[u];
+      }
     }
 
     // ---- partial or final output: thread = one d (and d + 128) of every head
@@ -461,7 +493,7 @@ __global__ void __launch_bounds__(192)
 #pragma unroll
     for (int h = 0; h < GP; h++) {
       l[h] = warp_sum(l[h]);
-      if (lane == 0 && h < G) wsum[warp * 8 + h] = l[h];
+      if (lane == 0 && has(h)) wsum[warp * 8 + h] = l[h];
     }
     ok = named_bar_and(1, 128, ok);
     if (ok) {
@@ -469,31 +501,31 @@ __global__ void __launch_bounds__(192)
       const bool split = n_chunks > 1;
 #pragma unroll
       for (int h = 0; h < GP; h++)
-        if (h < G) l[h] = (wsum[h] + wsum[8 + h]) + (wsum[16 + h] + wsum[24 + h]);
+        if (has(h)) l[h] = (wsum[h] + wsum[8 + h]) + (wsum[16 + h] + wsum[24 + h]);
 #pragma unroll
       for (int hb = 0; hb < C::HB; hb++) {
         uint32_t raw[N];
 #pragma unroll
         for (int i = 0; i < N; i += 16) tmem_ld16(tmem + lanes + C::O_COL + hb * N + i, raw + i);
         tmem_ld_wait();
-        const int d = hb * 128 + tid;
+        const int d = C::PAIR ? tid & 63 : hb * 128 + tid;
 #pragma unroll
         for (int h = 0; h < GP; h++) {
-          if (h >= G) continue;
-          float x = __uint_as_float(raw[h * P + P - 1]);
+          if (!has(h) || (C::PAIR && tid >> 6 != h / GH)) continue;
+          float x = __uint_as_float(raw[C::col(h, P - 1)]);
 #pragma unroll
-          for (int p = P - 2; p >= 0; p--) x = fmaf(x, 0.0625f, __uint_as_float(raw[h * P + p]));
+          for (int p = P - 2; p >= 0; p--) x = fmaf(x, 0.0625f, __uint_as_float(raw[C::col(h, p)]));
           x *= 1.f / kPScale;
-          if (split) a.ws_acc[(((int64_t)b * a.H + head0 + h) * a.cmax + ck) * HD + d] = x;
-          else st_any(a.o, b * a.o_bstride + (int64_t)(head0 + h) * HD + d, a.dtype_o, x / l[h]);
+          if (split) a.ws_acc[(((int64_t)b * a.H + head(h)) * a.cmax + ck) * HD + d] = x;
+          else st_any(a.o, b * a.o_bstride + (int64_t)head(h) * HD + d, a.dtype_o, x / l[h]);
         }
       }
       if (split) {
         if (tid == 0)
 #pragma unroll
           for (int h = 0; h < GP; h++)
-            if (h < G) {
-              float* ml = a.ws_ml + (((int64_t)b * a.H + head0 + h) * a.cmax + ck) * 2;
+            if (has(h)) {
+              float* ml = a.ws_ml + (((int64_t)b * a.H + head(h)) * a.cmax + ck) * 2;
               ml[0] = m[h];
               ml[1] = l[h];
             }
@@ -506,9 +538,12 @@ __global__ void __launch_bounds__(192)
         if (mine) {
           // the last CTA: merge the chunks, in their order
           __threadfence();
-          for (int h = 0; h < G; h++) {
-            const float* ml = a.ws_ml + ((int64_t)b * a.H + head0 + h) * a.cmax * 2;
-            const float* acc = a.ws_acc + ((int64_t)b * a.H + head0 + h) * a.cmax * HD;
+          const int half = C::PAIR ? tid >> 6 : 0, d = C::PAIR ? tid & 63 : tid;
+          for (int g = 0; g < G; g++) {
+            if (half >= halves) break;
+            const int h = head(half * GH + g);
+            const float* ml = a.ws_ml + ((int64_t)b * a.H + h) * a.cmax * 2;
+            const float* acc = a.ws_acc + ((int64_t)b * a.H + h) * a.cmax * HD;
             float M = -INFINITY;
             for (int c = 0; c < n_chunks; c++) M = fmaxf(M, __ldcg(ml + 2 * c));
             float L = 0.f, x[C::HB];
@@ -519,11 +554,11 @@ __global__ void __launch_bounds__(192)
               L = fmaf(__ldcg(ml + 2 * c + 1), w, L);
 #pragma unroll
               for (int hb = 0; hb < C::HB; hb++)
-                x[hb] = fmaf(__ldcg(acc + (int64_t)c * HD + hb * 128 + tid), w, x[hb]);
+                x[hb] = fmaf(__ldcg(acc + (int64_t)c * HD + hb * 128 + d), w, x[hb]);
             }
 #pragma unroll
             for (int hb = 0; hb < C::HB; hb++)
-              st_any(a.o, b * a.o_bstride + (int64_t)(head0 + h) * HD + hb * 128 + tid, a.dtype_o,
+              st_any(a.o, b * a.o_bstride + (int64_t)h * HD + hb * 128 + d, a.dtype_o,
                      x[hb] / L);
           }
           if (tid == 0) *cnt = 0u;
@@ -540,12 +575,16 @@ __global__ void __launch_bounds__(192)
   }
 }
 
-// 4-D map over B caches [max_seq][Hkv][hd] of bytes, box {128, 1, 128, 1}.
+// 4-D map over B caches [max_seq][Hkv][hd] of bytes, box {128, 1, 128, 1}; at
+// head_dim 64 a row's KV heads are one run of bytes, 128 of them a pair (an odd
+// last one's other half is filled with zeros).
 static bool make_kv8_map(CUtensorMap* m, const void* base, const Kv8DecodeArgs& a) {
   auto fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)a.hd, (cuuint64_t)a.hkv, (cuuint64_t)a.max_seq, (cuuint64_t)a.batch};
-  cuuint64_t strides[3] = {(cuuint64_t)a.hd, (cuuint64_t)a.hkv * a.hd,
+  const bool pair = a.hd == 64;
+  cuuint64_t dims[4] = {(cuuint64_t)(pair ? a.hd * a.hkv : a.hd), (cuuint64_t)(pair ? 1 : a.hkv),
+                        (cuuint64_t)a.max_seq, (cuuint64_t)a.batch};
+  cuuint64_t strides[3] = {dims[0], (cuuint64_t)a.hkv * a.hd,
                            a.batch > 1 ? (cuuint64_t)a.cache_bstride
                                        : (cuuint64_t)a.max_seq * a.hkv * a.hd};
   cuuint32_t box[4] = {128, 1, kKvTile, 1};
@@ -564,23 +603,25 @@ static cudaError_t run_kv8_tc(const Kv8DecodeArgs& a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   CUtensorMap mk, mv;
   if (!make_kv8_map(&mk, a.kcache, a) || !make_kv8_map(&mv, a.vcache, a)) return cudaErrorInvalidValue;
-  kern<<<dim3(a.hkv * a.gsubs, a.batch, a.cmax), 192, C::SMEM, st>>>(mk, mv, a);
+  kern<<<dim3((a.hkv + C::HALVES - 1) / C::HALVES * a.gsubs, a.batch, a.cmax), 192, C::SMEM, st>>>(mk, mv, a);
   return cudaGetLastError();
 }
 
 template <int HD, int P>
 static cudaError_t run_kv8_group(const Kv8DecodeArgs& a, cudaStream_t st) {
-  const int heads = a.H / a.hkv;
+  const int heads = a.H / a.hkv * (HD == 64 ? 2 : 1);
   if (heads > 4) return run_kv8_tc<HD, 8, P>(a, st);
   if (heads > 2) return run_kv8_tc<HD, 4, P>(a, st);
-  if (heads > 1) return run_kv8_tc<HD, 2, P>(a, st);
-  return run_kv8_tc<HD, 1, P>(a, st);
+  if constexpr (HD != 64)
+    if (heads == 1) return run_kv8_tc<HD, 1, P>(a, st);
+  return run_kv8_tc<HD, 2, P>(a, st);
 }
 
-bool kv8_tc_supported(int hd) { return hd == 128 || hd == 256; }
+bool kv8_tc_supported(int hd) { return hd == 64 || hd == 128 || hd == 256; }
 
 cudaError_t launch_kv8_decode_tc(const Kv8DecodeArgs& a, cudaStream_t st) {
   const bool wide = a.dtype_o == kF32;
+  if (a.hd == 64) return wide ? run_kv8_group<64, 5>(a, st) : run_kv8_group<64, 4>(a, st);
   if (a.hd == 128) return wide ? run_kv8_group<128, 5>(a, st) : run_kv8_group<128, 4>(a, st);
   return wide ? run_kv8_group<256, 5>(a, st) : run_kv8_group<256, 4>(a, st);
 }

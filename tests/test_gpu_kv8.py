@@ -292,6 +292,45 @@ def test_decode_block_scale_grows(eb):
             assert np.array_equal(got[n][0], c.np[n][0]) and np.array_equal(got[n][1], c.np[n][1]), (p, n)
 
 
+@pytest.mark.parametrize("H,heads", [(3, 3), (10, 5), (35, 7), (24, 3), (40, 4), (27, 3), (8, 8)])
+@pytest.mark.parametrize("f8,dtype", [("e4m3", "bf16"), ("e5m2", "f32")])
+def test_decode_neighbouring_heads(eb, H, heads, f8, dtype):
+    """head_dim 64, where two KV heads share a tile: odd numbers of them, one to ten query heads each."""
+    _decode(eb, positions=[333, 9, 128], H=H, heads=heads, hd=64, block=32, f8=f8, dtype=dtype, norm=True)
+
+
+@pytest.mark.parametrize("heads", [1, 2, 5])
+def test_decode_neighbouring_heads_split(eb, heads):
+    """As many rows as make several chunks, unequal lengths, a window that begins in the middle."""
+    for window in (0, 5000):
+        _decode(eb, positions=[9000, 17, 4095, 8191], H=4 * heads, heads=heads, hd=64, block=128, max_pos=9001,
+                max_seq=9100, window=window)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [0, 1, 2])
+def test_decode_nan_stays_in_its_head(eb, hd, bad):
+    """NaN in the rows of one KV head reaches the query heads of that one alone."""
+    import torch
+    heads, G, p = 3, 2, 200
+    c = _Cache(1, p + 1, heads, hd, 16, "e4m3", 1)
+    c.fill(0, p + 1, 2, 1.0)
+    desc = eb.make_desc(G * heads, heads, hd, p + 1, dtype_cache=eb.EB_E4M3)
+    ws = eb.alloc_workspace(eb.attention_decode_kv8_workspace_bytes(desc, 1, p))
+    q, outs = _dev(_randn(3, G * heads, hd)), []
+    for nan in (False, True):
+        if nan:
+            c.np["k"][0][0, 50, bad, 3] = 0x7F
+            c.np["v"][0][0, 60, bad] = 0x7F
+        o = torch.empty(G * heads, hd, device="cuda")
+        eb.attention_decode_kv8(desc, None, c.upload(eb), 1, torch.tensor([p], dtype=torch.int32, device="cuda"), p,
+                                q, None, None, o, ws)
+        outs.append(o.cpu().numpy().reshape(heads, G, hd))
+    rest = np.arange(heads) != bad
+    assert np.isnan(outs[1][bad]).all()
+    assert np.array_equal(outs[0][rest], outs[1][rest]) and np.isfinite(outs[0]).all()
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256, 40])
 def test_decode_garbage_behind_the_context(eb, hd):
     """Rows past the position hold NaN codes and NaN scales: nothing of them reaches o."""
