@@ -84,6 +84,7 @@ class Kv8(ctypes.Structure):
 
 class SampleParams(ctypes.Structure):
     """eb_sample_params: per-row temperature, top-k, top-p and min-p arrays."""
+    rows = 1 << 24  # that the arrays hold
     _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p),
                 ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p)]
 
@@ -292,6 +293,8 @@ def w4_quantize(w, group=128, zero_point=False, dtype_scale=EB_F16):
 def make_w4(q, scale, zero, in_f, out_f, group, dtype_scale=None):
     """eb_w4 over device tensors (kept alive by the object). The scale type is the scale
     tensor's unless dtype_scale says otherwise."""
+    _dtype(q, "u8", "make_w4: q")
+    _dtype(zero, "u8", "make_w4: zero")
     if dtype_scale is None:
         dtype_scale = torch_dtype_code(scale.dtype)
     w = W4(in_f, out_f, group, dtype_scale, _ptr(q), _ptr(scale), _ptr(zero))
@@ -303,17 +306,52 @@ def linear_w4_workspace_bytes(m, in_f, out_f) -> int:
     return lib().eb_linear_w4_workspace_bytes(m, in_f, out_f)
 
 
-def _row_stride(t) -> int:
-    return t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else 0
+def _refuse(what):
+    lib()
+    raise EbError(1, what)
+
+
+def _row_stride(t, shape, what) -> int:
+    """Stride of the rows of [rows, n] or of one row [n]; other layouts have none, nor do rows that
+    are one (an expanded tensor)."""
+    st = t.stride()
+    if len(st) == 2 and (st[1] == 1 or shape[1] < 2):
+        if shape[0] < 2:
+            return 0
+        if st[0] >= shape[1]:
+            return st[0]
+    elif len(st) == 1 and (st[0] == 1 or shape[0] < 2):
+        return 0
+    _refuse(f"{what}: rows of a tensor of shape {tuple(shape)}, strides {st}")
+
+
+_names = {}  # dtype -> its name
+
+
+def _dtype(t, name, what):
+    """Refuses a tensor of another type (u8: any of one byte)."""
+    if not hasattr(t, "element_size"):
+        return
+    have = _names.get(t.dtype)
+    if have is None:
+        have = _names[t.dtype] = "u8" if t.element_size() == 1 else str(t.dtype)[6:]
+    if have != name:
+        _refuse(f"{what}: {t.dtype}, not {name}")
 
 
 def linear_w4(w: W4, x, y, m, workspace=None, stream=None):
     """eb_linear_w4: y [m, out_f] = x [m, in_f] @ W^T with 4-bit weights; x and y are tensors in
-    f32, f16 or bf16 whose rows may be strided."""
+    f32, f16 or bf16 of [m, n] or, of one row, [n], whose rows may be strided."""
+    xs, ys = x.shape, y.shape
+    if (m > (xs[0] if len(xs) > 1 else 1) or m > (ys[0] if len(ys) > 1 else 1)
+            or xs[-1] < w.in_f or ys[-1] < w.out_f):
+        _refuse(f"linear_w4: {m} rows of {tuple(xs)} and {tuple(ys)}")
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _check(lib().eb_linear_w4(w, _ptr(x), torch_dtype_code(x.dtype), _row_stride(x), _ptr(y),
-                              torch_dtype_code(y.dtype), _row_stride(y), m, _ptr(workspace),
-                              ws_bytes, _stream(stream)), "eb_linear_w4")
+    _check(lib().eb_linear_w4(w, _ptr(x), torch_dtype_code(x.dtype),
+                              _row_stride(x, xs, "linear_w4"), _ptr(y),
+                              torch_dtype_code(y.dtype),
+                              _row_stride(y, ys, "linear_w4"), m, _ptr(workspace), ws_bytes,
+                              _stream(stream)), "eb_linear_w4")
 
 
 def rope_tables(max_seq: int, head_dim: int, theta: float, rope_angles: int | None = None):
@@ -458,6 +496,8 @@ def attention_decode_noalloc(desc, layer, pos, q, k, v, kcache, vcache, o, strea
 def make_kv8(k, v, k_scale, v_scale, block, batch_stride=0, scale_batch_stride=0):
     """eb_kv8 over device tensors (kept alive by the object): codes [(batch,) max_seq, kv_heads,
     head_dim] of one byte, scales f32 [(batch,) ceil(max_seq / block), kv_heads]."""
+    for t, name in ((k, "u8"), (v, "u8"), (k_scale, "float32"), (v_scale, "float32")):
+        _dtype(t, name, "make_kv8")
     c = Kv8(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), batch_stride, scale_batch_stride, block)
     c._keepalive = (k, v, k_scale, v_scale)
     return c
@@ -488,8 +528,14 @@ def attention_decode_kv8(desc, layer, cache: Kv8, batch, positions, max_pos, q, 
 def make_sample_params(temperature=None, top_k=None, top_p=None, min_p=None):
     """eb_sample_params over device arrays of one value per row (f32, top_k int32; None leaves a
     filter out), kept alive by the object."""
+    for t, name in ((temperature, "float32"), (top_k, "int32"), (top_p, "float32"), (min_p, "float32")):
+        _dtype(t, name, "make_sample_params")
+    given = [t for t in (temperature, top_k, top_p, min_p) if hasattr(t, "numel")]
+    if not all(t.is_contiguous() for t in given):
+        _refuse("make_sample_params: strided")
     p = SampleParams(_ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p))
     p._keepalive = (temperature, top_k, top_p, min_p)
+    p.rows = min((t.numel() for t in given), default=1 << 24)
     return p
 
 
@@ -500,10 +546,16 @@ def sample_workspace_bytes(rows, vocab) -> int:
 def sample(logits, params: SampleParams | None, u, ids, workspace=None, stream=None):
     """eb_sample: ids [rows] (int32) drawn from logits [rows, vocab] (or one row [vocab]) with the
     uniform numbers u [rows] (f32)."""
-    rows, vocab = logits.shape if logits.dim() == 2 else (1, logits.shape[0])
+    shape = logits.shape
+    rows, vocab = shape if len(shape) == 2 else (1, shape[0])
+    if (u.numel() < rows or ids.numel() < rows or (params is not None and params.rows < rows)
+            or not (u.is_contiguous() and ids.is_contiguous())):
+        _refuse(f"sample: {rows} rows, {u.numel()} uniform numbers, {ids.numel()} ids, or strided")
+    _dtype(u, "float32", "sample: u")
+    _dtype(ids, "int32", "sample: ids")
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _check(lib().eb_sample(_ptr(logits), torch_dtype_code(logits.dtype), rows, vocab,
-                           _row_stride(logits), params, _ptr(u), _ptr(ids), _ptr(workspace),
+                           _row_stride(logits, shape, "sample"), params, _ptr(u), _ptr(ids), _ptr(workspace),
                            ws_bytes, _stream(stream)), "eb_sample")
 
 

@@ -182,3 +182,37 @@ def test_valid_calls_without_a_device_are_refused(eb):
     assert L.eb_attention_decode_kv8(_desc(eb), None, _kv8(eb), 1, 16, 5, 16, 16, 16, 16, None, 0,
                                      None) == 5
     assert L.eb_sample(16, 0, 1, 100, 0, None, 16, 16, None, 0, None) == 5
+
+
+def test_binding_refuses_layouts_it_would_misread(eb):
+    """Tensors whose rows have no stride, are too short or too few, or are of another type: refused
+    before their pointers are taken."""
+    import torch
+    t = torch.zeros
+    w = eb.make_w4(t(64, 128, dtype=torch.uint8), t(4, 64, dtype=torch.float16), None, 256, 64, 64)
+    x, y = t(4, 256), t(4, 64)
+    for bad_x, bad_y, m in ((x, y, 5), (x[0], y, 2), (x, y[0], 2), (x[:1].expand(4, 256), y, 4), (x.t(), y, 4),
+                            (t(4, 512)[:, ::2], y, 4), (t(512)[::2], y, 1), (t(2, 2, 256), t(2, 2, 64), 2),
+                            (x[:, 1:], y, 4), (x, y[:, :63], 4), (x[0, :255], y[0], 1), (x, t(64, 4).t(), 4)):
+        with pytest.raises(eb.EbError) as e:
+            eb.linear_w4(w, bad_x, bad_y, m)
+        assert e.value.status == 1
+    logits, u, ids = t(4, 100), t(4), t(4, dtype=torch.int32)
+    short = eb.make_sample_params(t(3))
+    for args in ((logits.t(), None, t(100), t(100, dtype=torch.int32)), (logits[:1].expand(4, 100), None, u, ids),
+                 (t(4, 200)[:, ::2], None, u, ids), (logits, None, u[:3], ids), (logits, None, u, ids[:3]),
+                 (logits, None, u.double(), ids), (logits, None, u, ids.long()), (logits, short, u, ids),
+                 (logits, None, t(8)[::2], ids)):
+        with pytest.raises(eb.EbError) as e:
+            eb.sample(*args)
+        assert e.value.status == 1
+    for kw in (dict(temperature=t(4).double()), dict(top_k=t(4, dtype=torch.int64)), dict(top_p=t(4).half()),
+               dict(min_p=t(8)[::2])):
+        with pytest.raises(eb.EbError):
+            eb.make_sample_params(**kw)
+    k, s = t(64, 2, 64, dtype=torch.uint8), t(4, 2)
+    for args in ((k.float(), k, s, s), (k, k.half(), s, s), (k, k, s.half(), s), (k, k, s, s.double())):
+        with pytest.raises(eb.EbError):
+            eb.make_kv8(*args, 16)
+    with pytest.raises(eb.EbError):
+        eb.make_w4(t(64, 128), t(4, 64, dtype=torch.float16), None, 256, 64, 64)
