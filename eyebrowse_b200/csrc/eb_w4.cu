@@ -31,12 +31,14 @@ namespace eb {
 //
 // - The columns are three s8 planes of x: each (row of x, block of 128 inputs)
 //   is scaled by a power of two so that its largest value lies in [2^21, 2^22),
-//   rounded to a whole number (half a unit of f32's last place at the largest
-//   value, the only rounding), and split into bytes.
-// - A group's sum over its codes, less zero point times the sum of the same
-//   bytes, is exact in s32; it is turned to f32 (|sum| < 2^22: by adding it to
-//   the bits of 1.5 * 2^23), scaled by the group's scale and the plane's, and
-//   added to the row's f32 sum.
+//   rounded to a whole number (off by 2^-22 of the largest value at most), and
+//   split into bytes.
+// - A group's sum over its codes is exact in s32 and turned to f32 by adding it
+//   to the bits of 1.5 * 2^23 (|sum| < 2^22). One or two column tiles: zero
+//   point times the sum of the same bytes is taken off first, also exactly, and
+//   the planes' scales applied to each. Three: the planes are joined and the
+//   zero point's share taken off in f32. Then the group's scale, and the sum of
+//   the row in f32.
 // - The inputs of a k32 step may be any 32 as long as both operands agree, so
 //   the packed layout gives thread c of a quad 8 consecutive codes (one
 //   word) of each group of 32, even codes in one register, odd ones in the
@@ -46,6 +48,14 @@ namespace eb {
 //   walk over the tiles, so that x is staged once and the stream of weights
 //   does not stop between tiles. Partial sums meet in shared memory, then in
 //   the cluster's.
+//
+// Measured (calls in a row, weights from HBM; in brackets from L2 and out of a
+// graph, and there with f16 operands): one row by 4096 x 28672 22.5 us (16.5,
+// 26), eight rows by 14336 x 4096 27 us (23.5, 39), 37 rows by 4100 x 5003 in
+// groups of 32 49 us (45, 52), one row by 1024 x 4096 6.7 us (4.6, 4.8), which is
+// a launch, one trip to memory and the sums' two meetings. The large ones are
+// bound by issue slots: unpacking, and with eight rows the groups' sums (eight
+// f32 operations per output, group and plane triple).
 constexpr int kW4Ring = 2;   // pairs of blocks of a warp in its ring of shared memory
 constexpr int kW4Pair = 4096;  // bytes of a tile's pair of blocks
 constexpr int kW4Tile = 32;  // weight rows of a warp: two m16 tiles
@@ -496,6 +506,7 @@ size_t linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t) {
 // hold 21 clusters of 7).
 static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int* limit) {
   W4Plan p{};
+  const int sms = sm_count();
   const int64_t passes = (m + kW4Rows - 1) / kW4Rows;
   p.mt = w4_pass_rows(m);
   p.split_x = m > kW4Rows;
@@ -519,9 +530,9 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
       const int64_t grid = std::min(units, clusters) * split;
       const int64_t turns = (units + clusters - 1) / clusters;
       // an SM's CTAs; at most one of them has the last turn if few have
-      const int64_t per_sm = (grid * passes + sm_count() - 1) / sm_count();
+      const int64_t per_sm = (grid * passes + sms - 1) / sms;
       const int64_t last = (units - (turns - 1) * clusters) * split * passes;
-      const int64_t unit_sm = last <= sm_count() ? per_sm * (turns - 1) + 1 : per_sm * turns;
+      const int64_t unit_sm = last <= sms ? per_sm * (turns - 1) + 1 : per_sm * turns;
       const double blocks_warp = (double)((range + wk - 1) / wk);
       const double stage = (p.split_x ? 0.06 : 0.3) * (double)((range * 32 * p.mt + warps * 32 - 1) / (warps * 32));
       const double sums = split > 1 ? 0.6 : 0.3;
