@@ -32,8 +32,16 @@
 // and MMA issuer (S of tile j + 1 runs during the softmax of tile j). Chunks
 // start on multiples of 128 rows, so a block of rows never spans two; the CTA of
 // the last one appends the step's new row first (two warps each for K and V),
-// where one CTA has all heads of the KV head. The last CTA of a (sequence, head group) merges the chunks' partial (m, l, O) in chunk
-// order (atomic ticket, no spin-wait).
+// where one CTA has all heads of the KV head. The last CTA of a (sequence, head
+// group) merges the chunks' partial (m, l, O) in chunk order (atomic ticket, no
+// spin-wait).
+//
+// Measured: 64 sequences of 512 to 16384 rows, 8 KV heads of 128 with four query
+// heads each, 196 to 206 us, of which HBM needs 165: it is
+// bound by the softmax threads, four exponentials and four splits of a weight
+// into planes for each 256 bytes a row has. One sequence of 2048 rows 13 us: the
+// launch, the append, one trip to HBM, four barriers a tile and the merge.
+// head_dim 64: 64 sequences of 8192 rows, 8 KV heads, 124 us (the bytes need 82).
 #include "eb_kv8.cuh"
 #include "eb_rowops.cuh"
 #include "eb_tc.cuh"

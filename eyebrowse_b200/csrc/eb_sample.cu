@@ -28,7 +28,7 @@
 // results do not depend on timing (the list's order of arrival is undone by
 // the sort).
 //
-// A row is shared by a cluster of 1 to 8 CTAs; passes after the first read it
+// A row is shared by a cluster of 1 to 16 CTAs; passes after the first read it
 // from L1 or L2. What bounds it: for many open rows the f64 pipe (12
 // operations a token), for one row the chain of cluster barriers.
 #include <cooperative_groups.h>
@@ -416,319 +416,320 @@ __global__ void __launch_bounds__(kSampleThreads, 3) sample_kernel(SampleArgs a)
           if (b < kBins) count_up(&s.hist[b], 1);
         });
       }
-    __syncthreads();
-    if (C > 1) {
-      unsigned* to = cl.map_shared_rank(s.total, 0);
-      unsigned* to_place = cl.map_shared_rank(s.place_total, 0);
-      for (int i = tid; i < kBins; i += kSampleThreads)
-        if (s.hist[i]) {
-          atomicAdd(to + i, s.hist[i]);
-          if (sums) atomicAdd(to_place + i, s.place[i]);
-        }
-    }
-    sync();
-    const unsigned* total = C > 1 ? s.total : s.hist;
-    const unsigned* places = C > 1 ? s.place_total : s.place;
-    if (rank == 0) {
-      // some bins to a thread: counts and estimated masses, from the top. A
-      // bin's mass is taken as its count at the mean place of its tokens (plus
-      // what an even spread adds: (ln 2 / 32)^2 / 24).
-      constexpr int PER = (kBins + kSampleThreads - 1) / kSampleThreads;
-      unsigned cnt[PER], mine = 0, before, all;
-      double mass = 0, est[PER];
+      __syncthreads();
+      if (C > 1) {
+        unsigned* to = cl.map_shared_rank(s.total, 0);
+        unsigned* to_place = cl.map_shared_rank(s.place_total, 0);
+        for (int i = tid; i < kBins; i += kSampleThreads)
+          if (s.hist[i]) {
+            atomicAdd(to + i, s.hist[i]);
+            if (sums) atomicAdd(to_place + i, s.place[i]);
+          }
+      }
+      sync();
+      const unsigned* total = C > 1 ? s.total : s.hist;
+      const unsigned* places = C > 1 ? s.place_total : s.place;
+      if (rank == 0) {
+        // some bins to a thread: counts and estimated masses, from the top. A
+        // bin's mass is taken as its count at the mean place of its tokens (plus
+        // what an even spread adds: (ln 2 / 32)^2 / 24).
+        constexpr int PER = (kBins + kSampleThreads - 1) / kSampleThreads;
+        unsigned cnt[PER], mine = 0, before, all;
+        double mass = 0, est[PER];
 #pragma unroll
-      for (int j = 0; j < PER; j++) {
-        const int b = tid * PER + j;
-        cnt[j] = b < kBins ? total[b] : 0;
-        mine += cnt[j];
-        est[j] = 0;
-        if (sums && cnt[j]) {
-          const float mean = ((float)places[b] + 0.5f * cnt[j]) / (256.f * cnt[j]);
-          est[j] = cnt[j] * ex2_f64(-((double)b + (double)mean) / kPerOctave, s.tab) * (cnt[j] > 8 ? 1.0000195 : 1.0);
+        for (int j = 0; j < PER; j++) {
+          const int b = tid * PER + j;
+          cnt[j] = b < kBins ? total[b] : 0;
+          mine += cnt[j];
+          est[j] = 0;
+          if (sums && cnt[j]) {
+            const float mean = ((float)places[b] + 0.5f * cnt[j]) / (256.f * cnt[j]);
+            est[j] = cnt[j] * ex2_f64(-((double)b + (double)mean) / kPerOctave, s.tab) * (cnt[j] > 8 ? 1.0000195 : 1.0);
+          }
+          mass += est[j];
         }
-        mass += est[j];
-      }
-      before = block_scan(mine, s.warp_u, all);
-      double m_all, m_before = block_scan(mass, s.warp_d, m_all);
-      const bool k_cut = quick || (k_on && (unsigned)top_k < all);  // else fewer tokens have weight
-      const double want = sums ? (double)fmaxf(top_p, 0x1p-100f) * whole : 0.0;
-      if (tid == 0) {
-        s.lo = 0;
-        s.hi = kBins - 1;  // where no bin is the cut's
-      }
-      __syncthreads();
-      unsigned run = before;
-      double m_run = m_before;
-#pragma unroll
-      for (int j = 0; j < PER; j++) {  // the cut's bin
-        const bool here = k_cut ? run < (unsigned)top_k && run + cnt[j] >= (unsigned)top_k
-                                : m_run < want && m_run + est[j] >= want;
-        if (here && cnt[j]) atomicMin(&s.hi, tid * PER + j);
-        run += cnt[j];
-        m_run += est[j];
-      }
-      __syncthreads();
-      const int cut_bin = s.hi;
-      run = before;
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
-        if (tid * PER + j < kBins) s.offset[tid * PER + j] = (int)run;
-        if (tid * PER + j == cut_bin) {
-          s.above = run;
-          s.in = cnt[j];
+        before = block_scan(mine, s.warp_u, all);
+        double all_mass;
+        const double m_before = block_scan(mass, s.warp_d, all_mass);
+        const bool k_cut = quick || (k_on && (unsigned)top_k < all);  // else fewer tokens have weight
+        const double want = sums ? (double)fmaxf(top_p, 0x1p-100f) * whole : 0.0;
+        if (tid == 0) {
+          s.lo = 0;
+          s.hi = kBins - 1;  // where no bin is the cut's
         }
-        run += cnt[j];
-      }
-      __syncthreads();
-      const unsigned above = s.above, in = s.in;
-      int mode = kList;
-      if (quick) mode = all >= (unsigned)top_k ? kList : kAgain;
-      else if (!k_cut && !p_on) mode = kAll;
-      else if (in > kCap || (k_on && p_on && (k_cut ? above + in > kCap : all > kAround))) mode = kBisect;
-      else if (above + in > (k_cut ? kCap : kAround)) mode = kWide;
-      __syncthreads();
-      if (mode == kWide && tid == 0) s.lo = cut_bin;
-      __syncthreads();
-      // top_p's cut was estimated: take as many bins around as the list holds,
-      // below it first (half of the room left, in the wide case), then above
-      if (!k_cut && (mode == kList || mode == kWide)) {
-        const unsigned room = mode == kList ? kAround : above + in + (in < kAround ? (kAround - in) / 2 : 0);
+        __syncthreads();
+        unsigned run = before;
+        double m_run = m_before;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {  // the cut's bin
+          const bool here = k_cut ? run < (unsigned)top_k && run + cnt[j] >= (unsigned)top_k
+                                  : m_run < want && m_run + est[j] >= want;
+          if (here && cnt[j]) atomicMin(&s.hi, tid * PER + j);
+          run += cnt[j];
+          m_run += est[j];
+        }
+        __syncthreads();
+        const int cut_bin = s.hi;
         run = before;
 #pragma unroll
         for (int j = 0; j < PER; j++) {
+          if (tid * PER + j < kBins) s.offset[tid * PER + j] = (int)run;
+          if (tid * PER + j == cut_bin) {
+            s.above = run;
+            s.in = cnt[j];
+          }
           run += cnt[j];
-          const int b = tid * PER + j;
-          if (b > cut_bin && b < kBins && run <= room) atomicMax(&s.hi, b);
         }
         __syncthreads();
-        if (mode == kWide) {
-          const int hi = s.hi;
+        const unsigned above = s.above, in = s.in;
+        int mode = kList;
+        if (quick) mode = all >= (unsigned)top_k ? kList : kAgain;
+        else if (!k_cut && !p_on) mode = kAll;
+        else if (in > kCap || (k_on && p_on && (k_cut ? above + in > kCap : all > kAround))) mode = kBisect;
+        else if (above + in > (k_cut ? kCap : kAround)) mode = kWide;
+        __syncthreads();
+        if (mode == kWide && tid == 0) s.lo = cut_bin;
+        __syncthreads();
+        // top_p's cut was estimated: take as many bins around as the list holds,
+        // below it first (half of the room left, in the wide case), then above
+        if (!k_cut && (mode == kList || mode == kWide)) {
+          const unsigned room = mode == kList ? kAround : above + in + (in < kAround ? (kAround - in) / 2 : 0);
           run = before;
 #pragma unroll
           for (int j = 0; j < PER; j++) {
             run += cnt[j];
-            if (tid * PER + j == hi) s.in = run;  // tokens down to hi
-          }
-          __syncthreads();
-          const unsigned down = s.in;
-          run = before;
-#pragma unroll
-          for (int j = 0; j < PER; j++) {
             const int b = tid * PER + j;
-            if (b < cut_bin && down - run <= kAround) atomicMin(&s.lo, b);
-            run += cnt[j];
+            if (b > cut_bin && b < kBins && run <= room) atomicMax(&s.hi, b);
           }
           __syncthreads();
-        }
-      }
-      const int lo = s.lo, hi = s.hi;
-      if (tid < C) {
-        *at_rank(&s.mode, tid) = mode;
-        *at_rank(&s.lo, tid) = lo;
-        *at_rank(&s.hi, tid) = hi;
-        *at_rank(&s.k_cut, tid) = k_cut ? 1 : 0;
-      }
-    }
-    sync();
-    mode = s.mode;
-    int lo = s.lo, hi = s.hi;
-    const bool k_cut = s.k_cut != 0;
-    const float from_all = from;
-
-    for (int turn = 0; mode == kList || mode == kWide; turn++) {
-      // ---- pass 3: the window into rank 0's list, the sum (for top_k: the
-      // count) of what is above it
-      unsigned n_above = 0;
-      from = fmaxf(from_all, value_at((float)hi + 2.f));
-      above = 0;
-      const bool count = k_cut && lo > 0;
-      auto gather = [&](float l, int i, int b) {
-        if (b >= lo && b <= hi) {
-          const unsigned at = atomicAdd(&s.n_mine, 1u);
-          if (at < kCap) s.mine[at] = token_key(l, i);  // the window holds no more
-        }
-      };
-      if (lo == 0) {
-        each_token(row, i0, i1, from, [&](float l, int i) { gather(l, i, bin_of(l)); });
-      } else {
-        each_token(row, i0, i1, from, [&](float l, int i) {
-          const int b = bin_of(l);
-          gather(l, i, b);
-          if (b < lo) {
-            above += weight(l);
-            n_above++;
-          }
-        });
-        double all_a;
-        block_scan(count ? (double)n_above : above, s.warp_d, all_a);
-        if (tid == 0) *at_rank(&s.part[0][rank], 0) = all_a;
-      }
-      __syncthreads();
-      {
-        const unsigned have = s.n_mine;
-        if (tid == 0) s.base = atomicAdd(at_rank(&s.count, 0), have);
-        __syncthreads();
-        u64* list = at_rank(s.list, 0);
-        const unsigned base = s.base;
-        for (unsigned i = tid; i < have && i < kCap; i += kSampleThreads)
-          if (base + i < kCap) list[base + i] = s.mine[i];
-      }
-      sync();
-      if (rank == 0 && s.count > (quick ? kCount : kCap)) {  // a quick bound that was too low
-        if (tid < C) *at_rank(&s.mode, tid) = quick ? kAgain : kBisect;
-      } else if (rank == 0) {
-        const int m = (int)s.count;
-        // sorted: a short list by counting, a long one by bin (whose places
-        // pass 2 counted) and then within each bin
-        if (m <= kCount) {
-          sort_few(s.list, m);
-        } else {
-          const int start = s.offset[lo];
-          __syncthreads();
-          for (int i = tid; i < m; i += kSampleThreads) {
-            const u64 key = s.list[i];
-            const int b = bin_of(from_ordered((uint32_t)(key >> 32)));
-            const int at = atomicAdd(&s.offset[b], 1) - start;
-            if (at >= 0 && at < m) s.mine[at] = key;  // (always: the counts are these tokens')
-          }
-          __syncthreads();
-          for (int i = tid; i < m; i += kSampleThreads) {
-            const u64 key = s.mine[i];
-            const int b = bin_of(from_ordered((uint32_t)(key >> 32)));
-            const int end = min(s.offset[b] - start, m), begin = max(end - (int)total[b], 0);
-            int at = begin;
-            for (int j = begin; j < end; j++) at += s.mine[j] > key;
-            if (at < m) s.list[at] = key;
-          }
-          __syncthreads();
-          for (int b = lo + tid; b <= hi; b += kSampleThreads) s.offset[b] -= (int)total[b];
-        }
-        double over = 0;  // of what is above the window
-        if (lo > 0)
-          for (int q = 0; q < C; q++) over += s.part[0][q];
-        // running sums of the sorted list's weights, four to a thread
-        constexpr int PER = kCap / kSampleThreads;
-        double w[PER], mine = 0, all, b4[PER];
-        const int left = k_cut ? top_k - (count ? (int)over : 0) : m;  // places in the list
+          if (mode == kWide) {
+            const int hi = s.hi;
+            run = before;
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-          const int i = tid * PER + j;
-          w[j] = i < m && i < left ? weight(from_ordered((uint32_t)(s.list[i] >> 32))) : 0.0;
-          b4[j] = mine;
-          mine += w[j];
-        }
-        const double start = block_scan(mine, s.warp_d, all) + (sums ? over : 0.0);
-        if (!sums) whole = all;  // of the top_k tokens, or of all that have weight
-        const double want = (double)top_p * whole;
-        unsigned keep = 0, kept;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-          const int i = tid * PER + j;
-          const bool first = i == 0 && lo == 0;
-          if (i < m && i < left && (first || !p_on || count || start + b4[j] < want) &&
-              (first || w[j] >= min_p))
-            keep++;
-        }
-        block_scan(keep, s.warp_u, kept);
-        // top_p's cut is not in the window: above it, or below. The next window
-        // is as many of the bins there as the list holds.
-        const bool up = sums && lo > 0 && over >= want;
-        const bool down = sums && !up && (int)kept == m && hi + 1 < kBins && over + all < want;
-        if (up || down) {
-          mode = kShift;
-          __syncthreads();
-          if (tid == 0) {
-            s.lo = up ? lo : hi + 1;
-            s.hi = up ? lo - 1 : hi;
-          }
-          __syncthreads();
-          const int edge = up ? lo : hi + 1, tokens = s.offset[edge];
-          for (int b = tid; b < kBins; b += kSampleThreads) {
-            if (up && b < lo && tokens - s.offset[b] <= kCap) atomicMin(&s.lo, b);
-            if (down && b > hi && s.offset[b] + (int)total[b] - tokens <= kCap) atomicMax(&s.hi, b);
-          }
-          __syncthreads();
-          if (s.lo > s.hi || turn >= 8) mode = kBisect;  // a bin of more than the list holds
-        } else if ((int)kept > kCount && mode == kList) {
-          mode = kWide;  // pass 4 finds the token
-        }
-        if (mode == kList) {
-          // all kept tokens are here: in index order, the running sum again
-          u64 k2[PER];
-          __syncthreads();
-#pragma unroll
-          for (int j = 0; j < PER; j++) k2[j] = tid * PER + j < (int)kept ? s.list[tid * PER + j] : 0;
-          __syncthreads();
-#pragma unroll
-          for (int j = 0; j < PER; j++)  // complemented index first: descending is index ascending
-            if (tid * PER + j < (int)kept) s.list[tid * PER + j] = k2[j] << 32 | k2[j] >> 32;
-          sort_few(s.list, (int)kept);
-          mine = 0;
-#pragma unroll
-          for (int j = 0; j < PER; j++) {
-            const int i = tid * PER + j;
-            w[j] = i < (int)kept ? weight(from_ordered((uint32_t)s.list[i])) : 0.0;
-            mine += w[j];
-          }
-          double run = block_scan(mine, s.warp_d, all);
-          const double target = (double)u * all;
-          // the first place at which the sum passes the target
-#pragma unroll
-          for (int j = 0; j < PER; j++) {
-            const int i = tid * PER + j;
-            run += w[j];
-            if (w[j] > 0) {
-              if (run > target) atomicMin(&s.found, i);
-              atomicMax(&s.last, i);
+            for (int j = 0; j < PER; j++) {
+              run += cnt[j];
+              if (tid * PER + j == hi) s.in = run;  // tokens down to hi
             }
+            __syncthreads();
+            const unsigned down = s.in;
+            run = before;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+              const int b = tid * PER + j;
+              if (b < cut_bin && down - run <= kAround) atomicMin(&s.lo, b);
+              run += cnt[j];
+            }
+            __syncthreads();
           }
-          __syncthreads();
-          if (tid == 0) {
-            const int i = s.found < n ? s.found : s.last;
-            a.ids[r] = (int)(0xffffffffu - (uint32_t)(s.list[i] >> 32));
-          }
-        } else if (mode == kWide) {
-          // the last kept key; none in the window: what is above its first
-          if (tid == 0) s.cut = kept > 0 ? s.list[kept - 1] : m > 0 ? s.list[0] + 1 : ~0ull;
-          __syncthreads();
         }
+        const int lo = s.lo, hi = s.hi;
         if (tid < C) {
           *at_rank(&s.mode, tid) = mode;
-          *at_rank(&s.cut, tid) = s.cut;
-          const int to_lo = s.lo, to_hi = s.hi;
-          *at_rank(&s.lo, tid) = to_lo;
-          *at_rank(&s.hi, tid) = to_hi;
+          *at_rank(&s.lo, tid) = lo;
+          *at_rank(&s.hi, tid) = hi;
+          *at_rank(&s.k_cut, tid) = k_cut ? 1 : 0;
         }
       }
-      if (mode == kList) {
-        // rank 0 alone knows whether the list sufficed
-        sync();
-        if (s.mode == kList) return;
-      } else {
-        sync();
-      }
+      sync();
       mode = s.mode;
-      cut = s.cut;
-      if (mode == kShift) {
-        lo = s.lo;
-        hi = s.hi;
-        mode = kWide;
-        if (tid == 0) s.count = s.n_mine = 0;
+      int lo = s.lo, hi = s.hi;
+      const bool k_cut = s.k_cut != 0;
+      const float from_all = from;
+
+      for (int turn = 0; mode == kList || mode == kWide; turn++) {
+        // ---- pass 3: the window into rank 0's list, the sum (for top_k: the
+        // count) of what is above it
+        unsigned n_above = 0;
+        from = fmaxf(from_all, value_at((float)hi + 2.f));
+        above = 0;
+        const bool count = k_cut && lo > 0;
+        auto gather = [&](float l, int i, int b) {
+          if (b >= lo && b <= hi) {
+            const unsigned at = atomicAdd(&s.n_mine, 1u);
+            if (at < kCap) s.mine[at] = token_key(l, i);  // the window holds no more
+          }
+        };
+        if (lo == 0) {
+          each_token(row, i0, i1, from, [&](float l, int i) { gather(l, i, bin_of(l)); });
+        } else {
+          each_token(row, i0, i1, from, [&](float l, int i) {
+            const int b = bin_of(l);
+            gather(l, i, b);
+            if (b < lo) {
+              above += weight(l);
+              n_above++;
+            }
+          });
+          double all_a;
+          block_scan(count ? (double)n_above : above, s.warp_d, all_a);
+          if (tid == 0) *at_rank(&s.part[0][rank], 0) = all_a;
+        }
+        __syncthreads();
+        {
+          const unsigned have = s.n_mine;
+          if (tid == 0) s.base = atomicAdd(at_rank(&s.count, 0), have);
+          __syncthreads();
+          u64* list = at_rank(s.list, 0);
+          const unsigned base = s.base;
+          for (unsigned i = tid; i < have && i < kCap; i += kSampleThreads)
+            if (base + i < kCap) list[base + i] = s.mine[i];
+        }
         sync();
-        continue;
+        if (rank == 0 && s.count > (quick ? kCount : kCap)) {  // a quick bound that was too low
+          if (tid < C) *at_rank(&s.mode, tid) = quick ? kAgain : kBisect;
+        } else if (rank == 0) {
+          const int m = (int)s.count;
+          // sorted: a short list by counting, a long one by bin (whose places
+          // pass 2 counted) and then within each bin
+          if (m <= kCount) {
+            sort_few(s.list, m);
+          } else {
+            const int start = s.offset[lo];
+            __syncthreads();
+            for (int i = tid; i < m; i += kSampleThreads) {
+              const u64 key = s.list[i];
+              const int b = bin_of(from_ordered((uint32_t)(key >> 32)));
+              const int at = atomicAdd(&s.offset[b], 1) - start;
+              if (at >= 0 && at < m) s.mine[at] = key;  // (always: the counts are these tokens')
+            }
+            __syncthreads();
+            for (int i = tid; i < m; i += kSampleThreads) {
+              const u64 key = s.mine[i];
+              const int b = bin_of(from_ordered((uint32_t)(key >> 32)));
+              const int end = min(s.offset[b] - start, m), begin = max(end - (int)total[b], 0);
+              int at = begin;
+              for (int j = begin; j < end; j++) at += s.mine[j] > key;
+              if (at < m) s.list[at] = key;
+            }
+            __syncthreads();
+            for (int b = lo + tid; b <= hi; b += kSampleThreads) s.offset[b] -= (int)total[b];
+          }
+          double over = 0;  // of what is above the window
+          if (lo > 0)
+            for (int q = 0; q < C; q++) over += s.part[0][q];
+          // running sums of the sorted list's weights, four to a thread
+          constexpr int PER = kCap / kSampleThreads;
+          double w[PER], mine = 0, all, b4[PER];
+          const int left = k_cut ? top_k - (count ? (int)over : 0) : m;  // places in the list
+#pragma unroll
+          for (int j = 0; j < PER; j++) {
+            const int i = tid * PER + j;
+            w[j] = i < m && i < left ? weight(from_ordered((uint32_t)(s.list[i] >> 32))) : 0.0;
+            b4[j] = mine;
+            mine += w[j];
+          }
+          const double start = block_scan(mine, s.warp_d, all) + (sums ? over : 0.0);
+          if (!sums) whole = all;  // of the top_k tokens, or of all that have weight
+          const double want = (double)top_p * whole;
+          unsigned keep = 0, kept;
+#pragma unroll
+          for (int j = 0; j < PER; j++) {
+            const int i = tid * PER + j;
+            const bool first = i == 0 && lo == 0;
+            if (i < m && i < left && (first || !p_on || count || start + b4[j] < want) &&
+                (first || w[j] >= min_p))
+              keep++;
+          }
+          block_scan(keep, s.warp_u, kept);
+          // top_p's cut is not in the window: above it, or below. The next window
+          // is as many of the bins there as the list holds.
+          const bool up = sums && lo > 0 && over >= want;
+          const bool down = sums && !up && (int)kept == m && hi + 1 < kBins && over + all < want;
+          if (up || down) {
+            mode = kShift;
+            __syncthreads();
+            if (tid == 0) {
+              s.lo = up ? lo : hi + 1;
+              s.hi = up ? lo - 1 : hi;
+            }
+            __syncthreads();
+            const int edge = up ? lo : hi + 1, tokens = s.offset[edge];
+            for (int b = tid; b < kBins; b += kSampleThreads) {
+              if (up && b < lo && tokens - s.offset[b] <= kCap) atomicMin(&s.lo, b);
+              if (down && b > hi && s.offset[b] + (int)total[b] - tokens <= kCap) atomicMax(&s.hi, b);
+            }
+            __syncthreads();
+            if (s.lo > s.hi || turn >= 8) mode = kBisect;  // a bin of more than the list holds
+          } else if ((int)kept > kCount && mode == kList) {
+            mode = kWide;  // pass 4 finds the token
+          }
+          if (mode == kList) {
+            // all kept tokens are here: in index order, the running sum again
+            u64 k2[PER];
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; j++) k2[j] = tid * PER + j < (int)kept ? s.list[tid * PER + j] : 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; j++)  // complemented index first: descending is index ascending
+              if (tid * PER + j < (int)kept) s.list[tid * PER + j] = k2[j] << 32 | k2[j] >> 32;
+            sort_few(s.list, (int)kept);
+            mine = 0;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+              const int i = tid * PER + j;
+              w[j] = i < (int)kept ? weight(from_ordered((uint32_t)s.list[i])) : 0.0;
+              mine += w[j];
+            }
+            double run = block_scan(mine, s.warp_d, all);
+            const double target = (double)u * all;
+            // the first place at which the sum passes the target
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+              const int i = tid * PER + j;
+              run += w[j];
+              if (w[j] > 0) {
+                if (run > target) atomicMin(&s.found, i);
+                atomicMax(&s.last, i);
+              }
+            }
+            __syncthreads();
+            if (tid == 0) {
+              const int i = s.found < n ? s.found : s.last;
+              a.ids[r] = (int)(0xffffffffu - (uint32_t)(s.list[i] >> 32));
+            }
+          } else if (mode == kWide) {
+            // the last kept key; none in the window: what is above its first
+            if (tid == 0) s.cut = kept > 0 ? s.list[kept - 1] : m > 0 ? s.list[0] + 1 : ~0ull;
+            __syncthreads();
+          }
+          if (tid < C) {
+            *at_rank(&s.mode, tid) = mode;
+            *at_rank(&s.cut, tid) = s.cut;
+            const int to_lo = s.lo, to_hi = s.hi;
+            *at_rank(&s.lo, tid) = to_lo;
+            *at_rank(&s.hi, tid) = to_hi;
+          }
+        }
+        if (mode == kList) {
+          // rank 0 alone knows whether the list sufficed
+          sync();
+          if (s.mode == kList) return;
+        } else {
+          sync();
+        }
+        mode = s.mode;
+        cut = s.cut;
+        if (mode == kShift) {
+          lo = s.lo;
+          hi = s.hi;
+          mode = kWide;
+          if (tid == 0) s.count = s.n_mine = 0;
+          sync();
+          continue;
+        }
+        if (mode == kWide && min_p == 0.0) {
+          win_lo = lo;
+          win_hi = hi;
+        }
+        break;
       }
-      if (mode == kWide && min_p == 0.0) {
-        win_lo = lo;
-        win_hi = hi;
-      }
-      break;
-    }
-    if (mode != kAgain) break;
-    quick = false;
-    from = -INFINITY;
-    for (int i = tid; i < kBins; i += kSampleThreads) s.hist[i] = s.total[i] = 0;
-    if (tid == 0) s.count = s.n_mine = 0;
-    sync();
+      if (mode != kAgain) break;
+      quick = false;
+      from = -INFINITY;
+      for (int i = tid; i < kBins; i += kSampleThreads) s.hist[i] = s.total[i] = 0;
+      if (tid == 0) s.count = s.n_mine = 0;
+      sync();
     }
     if (mode == kBisect) {
       // ---- a pass per bit of the key: counts, then exact sums

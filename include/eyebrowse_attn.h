@@ -367,14 +367,15 @@ EB_API int eb_w4_quantize(const float* w, int64_t in_f, int64_t out_f, int32_t g
 
 /* y [m, out_f] = x [m, in_f] * W^T, beside eb_linear_f16w. x and y in f32, f16
  * or bf16, rows x_stride / y_stride elements apart (0 = in_f / out_f); x and y
- * do not overlap. Sums are in f32; 16-bit activations enter exactly, f32 ones
- * with 22 bits (and both without what lies below 2^-39 of the largest of 128
- * neighbouring inputs); a row with a value that is not finite yields NaN or
- * an infinity. Made for the few rows of decode steps: up to 24 rows of 16-bit
- * activations, or 12 of f32, stream the weights once, more rows once more for
- * each such number (from L2 where they fit). m <= 2^18, in_f and out_f <=
- * 2^24. eb_linear_w4_workspace_bytes is 0 for m <= 8. The workspace is
- * 256-byte aligned and needs no initialisation. */
+ * do not overlap. An activation enters as a whole number of units of a power
+ * of two, with an error of at most 2^-22 of the largest of its block of 128
+ * neighbouring inputs; sums are of whole numbers within a group and in f32
+ * beyond. A row with a value that is not finite yields NaN. Made for the few rows of decode steps: up to 8 rows stream the
+ * weights once, more rows once more for each 8 (from L2 where they fit).
+ * m <= 2^18, in_f and out_f <= 2^24. eb_linear_w4_workspace_bytes is 0 for
+ * m <= 8; above, the rows' whole numbers lie there. The workspace is 256-byte
+ * aligned and needs no initialisation; calls that share one must not overlap
+ * on the GPU. */
 EB_API size_t eb_linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t out_f);
 EB_API int eb_linear_w4(const eb_w4* w, const void* x, int32_t dtype_x, int64_t x_stride, void* y,
                         int32_t dtype_y, int64_t y_stride, int64_t m, void* workspace,
@@ -417,12 +418,16 @@ EB_API int eb_kv8_write(const eb_attn_desc* desc, const eb_attn_layer* layer, co
 
 /* eb_attention_decode_batched over an 8-bit cache: appends each sequence's new
  * k and v rows at positions[b] (k == v == NULL appends nothing) and attends
- * rows 0..=positions[b] (the last `window` of them) into o, in f32
- * arithmetic throughout. positions: DEVICE int32; a value outside [0,
+ * rows 0..=positions[b] (the last `window` of them) into o. Scores, softmax
+ * statistics and sums are in f32; at head_dim 64, 128 and 256 q and the
+ * weights enter the products with 20 bits where o is f32 and with 16 where o
+ * is a 16-bit type, else in f32. batch <= 32767. positions: DEVICE int32; a
+ * value outside [0,
  * max_pos] marks an empty slot of the batch, whose cache and output rows are
- * left as they are. positions == NULL: every sequence is at max_pos. Row
- * strides as for eb_attention_decode_batched; no alignment beyond the
- * element's for q, k, v and o. A workspace smaller than
+ * left as they are. positions == NULL: every sequence is at max_pos. No two
+ * sequences of a call share rows that it writes. Row strides as for
+ * eb_attention_decode_batched; no alignment beyond the element's for q, k, v
+ * and o. A workspace smaller than
  * eb_attention_decode_kv8_workspace_bytes is refused; it is zeroed once by
  * eb_workspace_init, each call leaves its counters at zero, and calls that
  * share one must not overlap on the GPU. */
@@ -458,7 +463,9 @@ typedef struct {
  * drawn. A NaN logit counts as -infinity, several +infinity as equals that
  * leave no weight to others. A row without a logit above -infinity gives -1.
  * u is clamped to [0, 1 - 2^-24], NaN to 0.
- * ids: DEVICE int32 [rows]. vocab <= 2^24. */
+ * ids: DEVICE int32 [rows]. rows and vocab <= 2^24. A row's scratch is in
+ * shared memory: eb_sample_workspace_bytes is 0 and the workspace may be
+ * NULL. */
 EB_API size_t eb_sample_workspace_bytes(int64_t rows, int64_t vocab);
 EB_API int eb_sample(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
                      int64_t row_stride, const eb_sample_params* params, const float* u,
