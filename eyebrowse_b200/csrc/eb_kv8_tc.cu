@@ -49,6 +49,7 @@
 namespace eb {
 
 constexpr int kKvTile = 128;
+constexpr int kKvChunks = 256;         // of a context, at most (the host's plan keeps to it)
 constexpr float kPScale = 32.f;        // P's plane 0 holds 32 * weight, at most 32 * 2^3.5 < 448
 constexpr float kKvRescale = 3.5f;
 constexpr float kMinLogScale = -64.f;  // of a V scale of zero
@@ -72,6 +73,7 @@ struct Kv8Cfg {
   static constexpr int SMEM = MISC_OFF + 512 + 1024;
   static constexpr int O_COL = 0, S_COL = HB * N;
   static constexpr int TMEM_COLS = constexpr_pow2ceil(HB * N + 2 * N);
+  static_assert(NST * 2 * K_BYTES >= GP * (kKvChunks + 1) * 4, "the merge's weights");
   static_assert(SMEM <= 232448 && TMEM_COLS <= 512 / (HB == 1 ? 2 : 1), "on-chip budgets");
 };
 
@@ -544,30 +546,48 @@ __global__ void __launch_bounds__(192)
         if (tid == 0) mine = atomicAdd(cnt, 1u) == (unsigned)(n_chunks - 1);
         mine = !named_bar_and(1, 128, !(tid == 0 && mine));
         if (mine) {
-          // the last CTA: merge the chunks, in their order
+          // The last CTA merges the chunks, in their order: weights by a warp per
+          // head, a chunk per lane, into the ring (nothing uses it any more);
+          // then a thread sums its d over them, eight loads in flight.
           __threadfence();
-          const int half = C::PAIR ? tid >> 6 : 0, d = C::PAIR ? tid & 63 : tid;
-          for (int g = 0; g < G; g++) {
-            if (half >= halves) break;
-            const int h = head(half * GH + g);
-            const float* ml = a.ws_ml + ((int64_t)b * a.H + h) * a.cmax * 2;
-            const float* acc = a.ws_acc + ((int64_t)b * a.H + h) * a.cmax * HD;
-            float M = -INFINITY;
-            for (int c = 0; c < n_chunks; c++) M = fmaxf(M, __ldcg(ml + 2 * c));
-            float L = 0.f, x[C::HB];
+          float* weight = reinterpret_cast<float*>(smem + C::KV_OFF);  // [GP][kKvChunks], then sums [GP]
+          for (int h = warp; h < GP; h += 4) {
+            if (!has(h)) continue;
+            const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + ((int64_t)b * a.H + head(h)) * a.cmax;
+            float2 v[kKvChunks / 32];
+            float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (int hb = 0; hb < C::HB; hb++) x[hb] = 0.f;
-            for (int c = 0; c < n_chunks; c++) {
-              const float w = ex2(__ldcg(ml + 2 * c) - M);
-              L = fmaf(__ldcg(ml + 2 * c + 1), w, L);
+            for (int i = 0; i < kKvChunks / 32; i++) {
+              v[i] = i * 32 + lane < n_chunks ? __ldcg(ml + i * 32 + lane) : make_float2(-INFINITY, 0.f);
+              M = fmaxf(M, v[i].x);
+            }
+            M = warp_max(M);
+#pragma unroll
+            for (int i = 0; i < kKvChunks / 32; i++) {
+              if (i * 32 + lane >= n_chunks) continue;
+              const float w = ex2(v[i].x - M);
+              weight[h * kKvChunks + i * 32 + lane] = w;
+              L = fmaf(v[i].y, w, L);
+            }
+            L = warp_sum(L);
+            if (lane == 0) weight[GP * kKvChunks + h] = L;
+          }
+          named_bar_and(1, 128, true);
+          const int half = C::PAIR ? tid >> 6 : 0, d = C::PAIR ? tid & 63 : tid;
+          for (int g = 0; g < G && half < halves; g++) {
+            const int h = half * GH + g;
+            const float* acc = a.ws_acc + ((int64_t)b * a.H + head(h)) * a.cmax * HD + d;
+            const float* w = weight + h * kKvChunks;
+            float x[C::HB] = {};
+#pragma unroll 8
+            for (int c = 0; c < n_chunks; c++)
 #pragma unroll
               for (int hb = 0; hb < C::HB; hb++)
-                x[hb] = fmaf(__ldcg(acc + (int64_t)c * HD + hb * 128 + d), w, x[hb]);
-            }
+                x[hb] = fmaf(__ldcg(acc + (int64_t)c * HD + hb * 128), w[c], x[hb]);
 #pragma unroll
             for (int hb = 0; hb < C::HB; hb++)
-              st_any(a.o, b * a.o_bstride + (int64_t)h * HD + hb * 128 + d, a.dtype_o,
-                     x[hb] / L);
+              st_any(a.o, b * a.o_bstride + (int64_t)head(h) * HD + hb * 128 + d, a.dtype_o,
+                     x[hb] / weight[GP * kKvChunks + h]);
           }
           if (tid == 0) *cnt = 0u;
         }
