@@ -266,6 +266,12 @@ def test_decode_many_rows_split(eb, hd):
     _decode(eb, positions=[9000, 17, 4095, 8191], H=8, heads=2, hd=hd, block=128, max_pos=9001, max_seq=9100)
 
 
+@pytest.mark.parametrize("hd,pos,H,heads", [(64, 131000, 3, 1), (128, 40000, 2, 1), (256, 40000, 6, 2), (64, 33000, 6, 3)])
+def test_decode_many_chunks(eb, hd, pos, H, heads):
+    """One long context in a hundred chunks and more, 256 of them in the first case."""
+    _decode(eb, positions=[pos], H=H, heads=heads, hd=hd, block=128, rope=False)
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256, 16])
 def test_decode_large_scores(eb, hd):
     """Scores of hundreds: one row takes nearly all the weight, wherever it stands."""
