@@ -183,7 +183,6 @@ struct Kv8WriteArgs {
   int max_pos;               // positions outside [0, max_pos] are skipped
   int block, hkv, hd, batch;
   bool e5m2;
-  bool aligned, tables_aligned;  // may be read in 16-byte words (set by the launcher)
   const float* k_norm_w;
   const float* v_norm_w;
   const float* cos_t;

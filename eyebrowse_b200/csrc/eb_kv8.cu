@@ -37,16 +37,19 @@ __device__ __forceinline__ float warp_sums(float (&s)[R], int lane) {
 // between finding their largest value and rounding them: a warp holds R rows,
 // E = head_dim / 32 neighbouring values of each per lane, all loaded before the
 // first is used, so every byte is read once and written once. 8192 rows of 8
-// heads of 128 in bf16 (50 MB), K normalised and rotated, take 27 us of which
-// HBM needs 8: it is bound by its instructions (900 a warp of eight rows, 58 %
-// of the issue slots) and, at three CTAs of 76 registers an SM, by the latency
-// of the one round of loads. So the norm's sums, roots and quotients are made
-// for eight rows at once (28 -> 27 us; a piece of 93 rows 6.1 -> 5.0 us).
-// kv8_write_kernel (any other head_dim) stages them as f32 in shared memory.
+// heads of 128 in bf16 (50 MB) take 19.4 us of which HBM needs 8. What bounds it
+// is the latency of that one round of loads, so the registers are held to 64 a
+// thread (with 76, three CTAs of 256 threads an SM instead of four, 25 us), and
+// the issue slots: addresses in 32 bits from a base, the norm's sums, roots and
+// quotients of eight rows at once.
+// kv8_write_kernel (any other head_dim, or rows and tables that do not start at
+// multiples of 16 bytes) stages them as f32 in shared memory: 57 us there. (With
+// both kinds of loads in the first kernel the second were issued as well, under
+// a predicate: 27 us instead of 25.)
 // CTAs of the same rows (K and V, every head) are neighbours: together they
 // read and write whole rows.
 template <typename T, int E, int R>
-__global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8WriteArgs a) {
+__global__ void __launch_bounds__(R >= 8 ? 512 : 1024, R >= 8 ? 2 : 1) kv8_write_rows_kernel(Kv8WriteArgs a) {
   constexpr int HD = 32 * E;
   __shared__ float warp_max_[32];
   const int which = blockIdx.x & 1, head = (int)((blockIdx.x >> 1) % a.hkv), b = blockIdx.y;
@@ -66,16 +69,19 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8
   const int before = (int)(lo - blk * a.block);  // rows of the block in front of the new ones
   const float old = before > 0 ? *scale : 0.f;
 
-  const T* src = static_cast<const T*>(which ? a.v : a.k) + b * a.kv_bstride + (int64_t)head * HD + lane * E;
+  // row r of the block: 32-bit products, 64-bit sums
+  const T* src = static_cast<const T*>(which ? a.v : a.k) + b * a.kv_bstride + (lo - start) * a.kv_stride +
+                 head * HD + lane * E;
+  const int src_stride = (int)a.kv_stride;
   const float* w = which ? a.v_norm_w : a.k_norm_w;
   const bool turn = !which && a.cos_t;
   // all loads first (a row past the end reads the last one again)
   RawRow<T, E> raw[R];
 #pragma unroll
   for (int i = 0; i < R; i++)
-    raw[i].load(src + (lo + min(i * warps + warp, n - 1) - start) * a.kv_stride, a.aligned);
+    raw[i].load(src + (int64_t)min(i * warps + warp, n - 1) * src_stride);
   RawRow<float, E> wr;
-  if (w) wr.load(w + lane * E, a.tables_aligned);
+  if (w) wr.load(w + lane * E);
   float v[R][E], amax = 0.f;
 #pragma unroll
   for (int i = 0; i < R; i++) raw[i].f32(v[i]);
@@ -100,11 +106,13 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8
   if (turn) {
     RawRow<float, E> tc[R], ts[R];
     const float sign = lane < 16 ? -1.f : 1.f;
+    const float* cos_t = a.cos_t + lo * (HD / 2) + (lane & 15) * E;
+    const float* sin_t = a.sin_t + lo * (HD / 2) + (lane & 15) * E;
 #pragma unroll
     for (int i = 0; i < R; i++) {
-      const int64_t at = (lo + min(i * warps + warp, n - 1)) * (HD / 2) + (lane & 15) * E;
-      tc[i].load(a.cos_t + at, a.tables_aligned);
-      ts[i].load(a.sin_t + at, a.tables_aligned);
+      const int at = min(i * warps + warp, n - 1) * (HD / 2);
+      tc[i].load(cos_t + at);
+      ts[i].load(sin_t + at);
     }
 #pragma unroll
     for (int i = 0; i < R; i++) {
@@ -130,32 +138,36 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024) kv8_write_rows_kernel(Kv8
 #pragma unroll
       for (int e = 0; e < E; e++) amax = f8_amax(amax, v[i][e]);
   }
-  amax = warp_max(amax);
+  // (floats that are not negative are in the order of their bits)
+  amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
   if (lane == 0) warp_max_[warp] = amax;
   __syncthreads();  // and every thread has read the old scale
-  for (int i = 0; i < warps; i++) amax = fmaxf(amax, warp_max_[i]);
+  amax = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(warp_max_[lane]) : 0u));
 
-  const int64_t stride = (int64_t)a.hkv * HD;
-  uint8_t* cache = static_cast<uint8_t*>(which ? a.vcache : a.kcache) + b * a.cache_bstride +
-                   (int64_t)head * HD;
+  const int stride = a.hkv * HD;
   float s = f8_need_scale(amax, a.e5m2);
   const bool grown = before > 0 && fmaxf(s, old) != old;
   if (before > 0) s = fmaxf(s, old);
-  const float inv = 1.0f / s, ratio = old / s;
-  uint8_t* first = cache + blk * a.block * stride + lane * E;
+  const float inv = 1.0f / s;
+  uint8_t* first = static_cast<uint8_t*>(which ? a.vcache : a.kcache) + b * a.cache_bstride +
+                   blk * a.block * stride + head * HD + lane * E;
   auto store = [&](auto e5m2) {
     constexpr bool E5M2 = decltype(e5m2)::value;
-    if (grown)  // the block's earlier rows, rounded again
+    if (grown) {  // the block's earlier rows, rounded again
+      const float ratio = old / s;
       for (int r = warp; r < before; r += warps) {
+        uint8_t* row = first + (int64_t)r * stride;
         float f[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) f[e] = f8_decode(first[r * stride + e], E5M2);
-        f8_store<E, E5M2>(first + r * stride, f, ratio);
+        for (int e = 0; e < E; e++) f[e] = f8_decode(row[e], E5M2);
+        f8_store<E, E5M2>(row, f, ratio);
       }
+    }
+    uint8_t* to = first + (int64_t)before * stride;
 #pragma unroll
     for (int i = 0; i < R; i++) {
       const int r = i * warps + warp;
-      if (r < n) f8_store<E, E5M2>(first + (before + r) * stride, v[i], inv);
+      if (r < n) f8_store<E, E5M2>(to + (int64_t)r * stride, v[i], inv);
     }
   };
   if (a.e5m2) store(std::true_type{});
@@ -225,13 +237,14 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
 template <typename T, int E>
 static void write_rows(const Kv8WriteArgs& a, int64_t per, cudaStream_t st) {
   const dim3 grid((unsigned)(per * a.hkv * 2), a.batch);
-  // Rows of a warp: eight where there are enough CTAs to fill the SMs, fewer in
-  // short pieces (93 rows of 4 heads of 256, normalised: 9.1 us with eight,
-  // 3.7 with two); a decode step's row takes one of four warps, the
-  // others are for rows that may be rounded again.
+  // Rows of a warp: eight (of 256 values four) where there are enough CTAs to
+  // fill the SMs, fewer in short pieces (93 rows of 4 heads of 256, normalised:
+  // 9.1 us with eight, 4.8 with two); a decode step's row takes one of four
+  // warps, the others are for rows that may be rounded again.
+  constexpr int R = E == 8 ? 4 : 8;
   const int64_t ctas = per * a.hkv * 2 * a.batch;
   if (a.count == 1) kv8_write_rows_kernel<T, E, 1><<<grid, 128, 0, st>>>(a);
-  else if (ctas >= 2 * sm_count()) kv8_write_rows_kernel<T, E, 8><<<grid, 4 * a.block, 0, st>>>(a);
+  else if (ctas >= 2 * sm_count()) kv8_write_rows_kernel<T, E, R><<<grid, 32 * a.block / R, 0, st>>>(a);
   else if (a.block <= 64) kv8_write_rows_kernel<T, E, 2><<<grid, 16 * a.block, 0, st>>>(a);
   else kv8_write_rows_kernel<T, E, 4><<<grid, 8 * a.block, 0, st>>>(a);
 }
@@ -247,11 +260,10 @@ cudaError_t launch_kv8_write(const Kv8WriteArgs& a0, cudaStream_t st) {
   Kv8WriteArgs a = a0;
   const int es = a.dtype_kv == kF32 ? 4 : 2;
   auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-  a.aligned = ((bits(a.k) | bits(a.v) | (uintptr_t)(a.kv_stride * es) |
-                (uintptr_t)(a.kv_bstride * es)) & 15) == 0;
-  a.tables_aligned = ((bits(a.cos_t) | bits(a.sin_t) | bits(a.k_norm_w) | bits(a.v_norm_w)) & 15) == 0;
+  const bool aligned = ((bits(a.k) | bits(a.v) | (uintptr_t)(a.kv_stride * es) | (uintptr_t)(a.kv_bstride * es) |
+                         bits(a.cos_t) | bits(a.sin_t) | bits(a.k_norm_w) | bits(a.v_norm_w)) & 15) == 0;
   const int64_t per = a.positions ? 1 : (a.start + a.count - 1) / a.block - a.start / a.block + 1;
-  if (a.hd == 64 || a.hd == 128 || a.hd == 256) {
+  if (aligned && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
     if (per * a.hkv * 2 > INT32_MAX) return cudaErrorNotSupported;
     if (a.dtype_kv == kF32) write_rows_hd<float>(a, per, st);
     else if (a.dtype_kv == kF16) write_rows_hd<__half>(a, per, st);

@@ -51,33 +51,27 @@ __device__ __forceinline__ void f8_store(uint8_t* p, const float (&v)[E], float 
   else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
-// E neighbouring elements: one or two loads where `aligned`, as they lie.
+// E neighbouring elements at a multiple of their size: one or two loads.
 template <typename T, int E>
 struct RawRow {
   static constexpr int W = E * (int)sizeof(T) / 4;
   uint32_t w[W];
-  __device__ __forceinline__ void load(const T* p, bool aligned) {
-    if (aligned) {
-      if constexpr (W == 1) {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-      } else if constexpr (W == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x;
-        w[1] = u.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < W; i += 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
-          w[i] = u.x;
-          w[i + 1] = u.y;
-          w[i + 2] = u.z;
-          w[i + 3] = u.w;
-        }
-      }
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (W == 1) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (W == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x;
+      w[1] = u.y;
     } else {
-      T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-      for (int i = 0; i < E; i++) e[i] = p[i];
+      for (int i = 0; i < W; i += 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+        w[i] = u.x;
+        w[i + 1] = u.y;
+        w[i + 2] = u.z;
+        w[i + 3] = u.w;
+      }
     }
   }
   __device__ __forceinline__ void f32(float (&f)[E]) const {
