@@ -52,8 +52,9 @@ template <typename T, int E, int R>
 __global__ void __launch_bounds__(R >= 8 ? 512 : 1024, R >= 8 ? 2 : 1) kv8_write_rows_kernel(Kv8WriteArgs a) {
   constexpr int HD = 32 * E;
   __shared__ float warp_max_[32];
-  const int which = blockIdx.x & 1, head = (int)((blockIdx.x >> 1) % a.hkv), b = blockIdx.y;
-  const int64_t blk0 = (blockIdx.x >> 1) / a.hkv;
+  const unsigned at_block = (blockIdx.x >> 1) / (unsigned)a.hkv;
+  const int which = blockIdx.x & 1, head = (int)((blockIdx.x >> 1) - at_block * a.hkv), b = blockIdx.y;
+  const int shift = 31 - __clz(a.block);  // a power of two
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t start = a.start;
   if (a.positions) {
@@ -62,11 +63,11 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024, R >= 8 ? 2 : 1) kv8_write
     start = p;
   }
   const int64_t end = start + a.count;
-  const int64_t blk = start / a.block + blk0;
-  const int64_t lo = max(start, blk * a.block), hi = min(end, (blk + 1) * a.block);
+  const int64_t blk = (start >> shift) + at_block;
+  const int64_t lo = max(start, blk << shift), hi = min(end, (blk + 1) << shift);
   const int n = (int)(hi - lo);
   float* scale = (which ? a.v_scale : a.k_scale) + b * a.scale_bstride + blk * a.hkv + head;
-  const int before = (int)(lo - blk * a.block);  // rows of the block in front of the new ones
+  const int before = (int)(lo - (blk << shift));  // rows of the block in front of the new ones
   const float old = before > 0 ? *scale : 0.f;
 
   // row r of the block: 32-bit products, 64-bit sums
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024, R >= 8 ? 2 : 1) kv8_write
   if (before > 0) s = fmaxf(s, old);
   const float inv = 1.0f / s;
   uint8_t* first = static_cast<uint8_t*>(which ? a.vcache : a.kcache) + b * a.cache_bstride +
-                   blk * a.block * stride + head * HD + lane * E;
+                   (blk << shift) * stride + head * HD + lane * E;
   auto store = [&](auto e5m2) {
     constexpr bool E5M2 = decltype(e5m2)::value;
     if (grown) {  // the block's earlier rows, rounded again
@@ -166,8 +167,8 @@ __global__ void __launch_bounds__(R >= 8 ? 512 : 1024, R >= 8 ? 2 : 1) kv8_write
     uint8_t* to = first + (int64_t)before * stride;
 #pragma unroll
     for (int i = 0; i < R; i++) {
-      const int r = i * warps + warp;
-      if (r < n) f8_store<E, E5M2>(to + (int64_t)r * stride, v[i], inv);
+      // (past the end: the last row again, the same bytes)
+      f8_store<E, E5M2>(to + (int64_t)min(i * warps + warp, n - 1) * stride, v[i], inv);
     }
   };
   if (a.e5m2) store(std::true_type{});
