@@ -155,6 +155,39 @@ def test_write_norm_rope_strided(eb, dtype, hd, block, start, count):
         assert np.array_equal(got[n][0][0, rest], codes[0, rest])
 
 
+@pytest.mark.parametrize("hd,heads", [(64, 3), (128, 2), (256, 2)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift,stride", [(1, 0), (0, 1), (3, 2)])
+def test_write_unaligned(eb, hd, heads, dtype, shift, stride):
+    """Rows that begin at any element, tables too: the same codes and scales, twice in a row."""
+    import torch
+    start, count, block, max_seq, row = 21, 60, 32, 100, heads * hd + stride
+    c = _Cache(1, max_seq, heads, hd, block, "e4m3", 3)
+    c.fill(0, start, 5, 0.25)
+    cache = c.upload(eb)
+    buf = [_dev(_randn(8 + i, shift + max_seq * row), dtype) for i in range(2)]
+    rows = [t[shift:shift + count * row].reshape(count, row) for t in buf]
+    cos, sin = (_dev(np.concatenate([np.zeros(shift, np.float32), t.ravel()]))[shift:] for t in _tables(max_seq, hd))
+    desc = eb.make_desc(heads, heads, hd, max_seq, dtype_qkv=eb.torch_dtype_code(buf[0].dtype),
+                        dtype_cache=eb.EB_E4M3, eps=EPS, kv_stride=row)
+    layer = eb.make_layer(None, None, None, cos, sin)
+    x = [t[:, :heads * hd].double().cpu().numpy().reshape(count, heads, hd) for t in rows]
+    ct, st = (t[start:start + count, None].astype(np.float64) for t in _tables(max_seq, hd))
+    x[0] = qo.row_rope(x[0], ct, st)
+    for _ in range(2):
+        eb.kv8_write(desc, layer, cache, start, count, rows[0], rows[1])
+    torch.cuda.synchronize()
+    got = c.download()
+    for n, t in zip("kv", x):
+        codes, scale = c.np[n]
+        qo.kv8_write(codes[0], scale[0], start, t, block, "e4m3")
+        assert np.array_equal(got[n][1], scale), n
+        s = scale[0][np.arange(start, start + count) // block][:, :, None]
+        _near(got[n][0][0, start:start + count], s, t, "e4m3", (hd + 8) * 2.0 ** -23 * np.abs(t).max(-1, keepdims=True))
+        rest = np.r_[0:start, start + count:max_seq]
+        assert np.array_equal(got[n][0][0, rest], codes[0, rest])
+
+
 # ---------------------------------------------------------------- decode
 def _decode(eb, *, positions, H, heads, hd, block, f8="e4m3", dtype="f32", o_dtype=None, max_seq=None,
             window=0, norm=False, rope=True, append=True, pad=0, fused=False, max_pos=None, scale=None,
