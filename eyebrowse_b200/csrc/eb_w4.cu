@@ -37,8 +37,8 @@ namespace eb {
 //   to the bits of 1.5 * 2^23 (|sum| < 2^22). One or two column tiles: zero
 //   point times the sum of the same bytes is taken off first, also exactly, and
 //   the planes' scales applied to each. Three: the planes are joined and the
-//   zero point's share taken off in f32. Then the group's scale, and the sum of
-//   the row in f32.
+//   zero point's share taken off, in groups of 32 in s32 (32 * 15 * 2^22 < 2^31),
+//   of more in f32. Then the group's scale, and the sum of the row in f32.
 // - The inputs of a k32 step may be any 32 as long as both operands agree, so
 //   the packed layout gives thread c of a quad 8 consecutive codes (one
 //   word) of each group of 32, even codes in one register, odd ones in the
@@ -52,7 +52,7 @@ namespace eb {
 // Measured (calls in a row, weights from HBM; in brackets from L2 and out of a
 // graph, and there with f16 operands): one row by 4096 x 28672 22.5 us (16.5,
 // 26), eight rows by 14336 x 4096 27 us (23.5, 39), 37 rows by 4100 x 5003 in
-// groups of 32 49 us (45, 52), one row by 1024 x 4096 6.7 us (4.6, 4.8), which is
+// groups of 32 45 us (41, 52; joined in f32 49), one row by 1024 x 4096 6.7 us (4.6, 4.8), which is
 // a launch, one trip to memory and the sums' two meetings. The large ones are
 // bound by issue slots: unpacking, and with eight rows the groups' sums (eight
 // f32 operations per output, group and plane triple).
@@ -153,7 +153,8 @@ __device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0
   float* at_group = sums + lane / (GROUP / 8) * sum_stride;
   if constexpr (JOINT) {
     if (lane % (GROUP / 8) == 0)
-      *at_group = fmaf((float)sum[0], 65536.f, fmaf((float)sum[1], 256.f, (float)sum[2]));
+      *at_group = GROUP == 32 ? __int_as_float(sum[0] * 65536 + sum[1] * 256 + sum[2])
+                              : fmaf((float)sum[0], 65536.f, fmaf((float)sum[1], 256.f, (float)sum[2]));
     if (lane == 0) *scale = unit(2);
   } else {
 #pragma unroll
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
               for (int t = 0; t < NT; t++) {
                 if (first)
 #pragma unroll
-                  for (int e = 0; e < 4; e++) sum[rt][t][e] = kMagic;
+                  for (int e = 0; e < 4; e++) sum[rt][t][e] = JOINT && GROUP == 32 ? 0 : kMagic;
                 mma_u8s8(sum[rt][t], f, h ? x[t].z : x[t].x, h ? x[t].w : x[t].y);
               }
             }
@@ -384,7 +385,16 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
                   s[r] = w4_scale(m & 0xffffu, sbf);
                   z[r] = (int)(m >> 16);
                 }
-                if constexpr (JOINT) {
+                if constexpr (JOINT && GROUP == 32) {
+                  const float2 b2 = *reinterpret_cast<const float2*>(bs + k * XC);
+                  const int2 z2 = *reinterpret_cast<const int2*>(bz + g * XC);
+#pragma unroll
+                  for (int e = 0; e < 4; e++) {
+                    const int whole = (sum[rt][0][e] * 256 + sum[rt][1][e]) * 256 + sum[rt][2][e] -
+                                      z[e >> 1] * (e & 1 ? z2.y : z2.x);
+                    acc[rt][0][e] = fmaf((float)whole, s[e >> 1] * (e & 1 ? b2.y : b2.x), acc[rt][0][e]);
+                  }
+                } else if constexpr (JOINT) {
                   const float2 b2 = *reinterpret_cast<const float2*>(bs + k * XC);
                   const float2 z2 = *reinterpret_cast<const float2*>(bz + g * XC);
 #pragma unroll
