@@ -67,7 +67,7 @@ struct Kv8Cfg {
   static constexpr int K_BYTES = HB * TILE;
   static constexpr int Q_OFF = 0, P_OFF = HB * ROWS, KV_OFF = P_OFF + 2 * ROWS;
   // two CTAs on an SM at head_dim 128, one at 256
-  static constexpr int NST = HB == 2 ? 3 : (KV_OFF + 6 * K_BYTES + 3072 <= 113 * 1024 ? 3 : 2);
+  static constexpr int NST = HB == 2 ? 3 : (KV_OFF + 6 * K_BYTES <= 110 * 1024 ? 3 : 2);
   static constexpr int BAR_OFF = KV_OFF + NST * 2 * K_BYTES;
   static constexpr int MISC_OFF = BAR_OFF + 256;  // warp maxima [2][4][8], sums [4][8], flags
   static constexpr int SMEM = MISC_OFF + 512 + 1024;
