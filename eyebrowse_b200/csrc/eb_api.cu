@@ -100,12 +100,22 @@ struct DecodePlan {
 static int64_t decode_target_ctas() { return (int64_t)EB_DECODE_CTAS_PER_SM * sm_count(); }
 
 // Split-K workspace layout for p.cmax chunks: combine tickets, then the
-// per-chunk (max, sum) pairs, then the per-chunk partial outputs.
+// per-chunk (max, sum) pairs, then the per-chunk partial outputs. The first
+// kTicketBytes hold tickets in every call, whatever its batch and heads, so that
+// no call's partials lie where another's tickets are and a workspace that was
+// zeroed once serves calls of all shapes. Tickets past them (more than 16384
+// (sequence, head group) pairs) are cleared by the call itself.
 static void decode_layout(DecodePlan& p, int64_t batch, int64_t h, int64_t hd) {
   p.cnt_off = 0;
-  p.ml_off = round_up((size_t)batch * h * sizeof(unsigned));
+  p.ml_off = std::max(kTicketBytes, round_up((size_t)batch * h * sizeof(unsigned)));
   p.acc_off = p.ml_off + round_up((size_t)batch * h * p.cmax * 2 * sizeof(float));
   p.bytes = p.acc_off + round_up((size_t)batch * h * p.cmax * hd * sizeof(float));
+}
+
+static cudaError_t clear_far_tickets(void* ws, int64_t tickets, cudaStream_t st) {
+  const size_t bytes = (size_t)tickets * sizeof(unsigned);
+  if (bytes <= kTicketBytes) return cudaSuccess;
+  return cudaMemsetAsync(static_cast<char*>(ws) + kTicketBytes, 0, bytes - kTicketBytes, st);
 }
 
 static DecodePlan plan_decode(int64_t batch, int64_t h, int64_t hkv, int64_t hd, int dtype_cache,
@@ -277,6 +287,8 @@ int decode_impl(const eb_attn_desc* d, const eb_attn_layer* L, int64_t batch,
     a.eps = d->eps;
     a.scale_log2 = d->scale * kLog2e;
     if (p.cmax > 1) {
+      const cudaError_t e = clear_far_tickets(ws, batch * d->n_heads, st);
+      if (e != cudaSuccess) return cuda_status(e);
       char* w = static_cast<char*>(ws);
       a.ws_cnt = reinterpret_cast<unsigned*>(w + p.cnt_off);
       a.ws_ml = reinterpret_cast<float*>(w + p.ml_off);
@@ -1126,6 +1138,8 @@ int eb_attention_decode_kv8(const eb_attn_desc* d, const eb_attn_layer* L, const
   a.chunk = p.chunk;
   a.cmax = p.cmax;
   if (p.cmax > 1) {
+    const cudaError_t e = clear_far_tickets(workspace, batch * d->n_heads, st);
+    if (e != cudaSuccess) return cuda_status(e);
     char* base = static_cast<char*>(workspace);
     a.ws_cnt = reinterpret_cast<unsigned*>(base + w.cnt_off);
     a.ws_ml = reinterpret_cast<float*>(base + w.ml_off);

@@ -12,6 +12,8 @@ namespace eb {
 // Destinations of a head gather (prefill and decode): at most this many
 // buffers, this GPU's and its peers'.
 constexpr int kMaxGather = 8;
+// Front of a decode workspace that holds nothing but split-K tickets (16384).
+constexpr size_t kTicketBytes = 64 * 1024;
 
 // Lets `kern` use `bytes` of dynamic shared memory on the current device: one
 // runtime call per kernel and device, remembered in *configured.

@@ -271,13 +271,15 @@ EB_API size_t eb_attention_decode_workspace_bytes(const eb_attn_desc* desc, int6
                                            int64_t max_pos);
 
 /* Zero a decode workspace once after allocating it: the split-K combine
- * counters it holds must start at zero (each call leaves them at zero).
- * Calls that share one workspace must not overlap on the GPU. */
+ * counters it holds must start at zero (each call leaves them at zero). One
+ * workspace serves calls of any batch, head counts and decode entry point that
+ * it is large enough for. Calls that share one must not overlap on the GPU, and
+ * only decode calls may use it (others' scratch would overwrite the counters). */
 EB_API int eb_workspace_init(void* workspace, size_t workspace_bytes, eb_stream_t stream);
 
 /* Size in bytes of the device scratch eb_attention_decode_noalloc owns on
  * every GPU that loads this library. */
-#define EB_NOALLOC_SCRATCH_BYTES (8u << 20)
+#define EB_NOALLOC_SCRATCH_BYTES ((8u << 20) + (64u << 10))
 
 /* eb_attention_decode without a workspace argument, for callers that cannot
  * allocate device memory: a plugin inside a host framework that owns the
@@ -429,8 +431,9 @@ EB_API int eb_kv8_write(const eb_attn_desc* desc, const eb_attn_layer* layer, co
  * eb_attention_decode_batched; no alignment beyond the element's for q, k, v
  * and o. A workspace smaller than
  * eb_attention_decode_kv8_workspace_bytes is refused; it is zeroed once by
- * eb_workspace_init, each call leaves its counters at zero, and calls that
- * share one must not overlap on the GPU. */
+ * eb_workspace_init, each call leaves its counters at zero, whatever its batch
+ * and head counts, so one workspace serves every decode call that it is large
+ * enough for, and calls that share one must not overlap on the GPU. */
 EB_API size_t eb_attention_decode_kv8_workspace_bytes(const eb_attn_desc* desc, int64_t batch,
                                                       int64_t max_pos);
 EB_API int eb_attention_decode_kv8(const eb_attn_desc* desc, const eb_attn_layer* layer,
