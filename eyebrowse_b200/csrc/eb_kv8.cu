@@ -273,11 +273,10 @@ cudaError_t launch_kv8_write(const Kv8WriteArgs& a0, cudaStream_t st) {
   }
   const int rows = (int)(a.count < a.block ? a.count : a.block);
   const size_t smem = (size_t)rows * a.hd * sizeof(float);
-  if (smem > 48 * 1024) {
-    static unsigned configured = 0;
-    const cudaError_t e = allow_smem(kv8_write_kernel, 128 * 256 * 4, &configured);
-    if (e != cudaSuccess) return e;
-  }
+  // (asked for at any size: the kernel's static shared memory counts too)
+  static unsigned configured = 0;
+  const cudaError_t e = allow_smem(kv8_write_kernel, 128 * 256 * 4, &configured);
+  if (e != cudaSuccess) return e;
   kv8_write_kernel<<<dim3((unsigned)per, a.hkv, 2 * a.batch), 256, smem, st>>>(a);
   return cudaGetLastError();
 }
