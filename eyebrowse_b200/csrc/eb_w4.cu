@@ -33,12 +33,14 @@ namespace eb {
 //   is scaled by a power of two so that its largest value lies in [2^21, 2^22),
 //   rounded to a whole number (off by 2^-22 of the largest value at most), and
 //   split into bytes.
-// - A group's sum over its codes is exact in s32 and turned to f32 by adding it
-//   to the bits of 1.5 * 2^23 (|sum| < 2^22). One or two column tiles: zero
-//   point times the sum of the same bytes is taken off first, also exactly, and
-//   the planes' scales applied to each. Three: the planes are joined and the
-//   zero point's share taken off, in groups of 32 in s32 (32 * 15 * 2^22 < 2^31),
-//   of more in f32. Then the group's scale, and the sum of the row in f32.
+// - A group's sum over its codes is exact in s32, and zero point times the sum of
+//   the same bytes is taken off it there, while nothing is rounded: both can be
+//   far larger than what they leave. Sums below 2^22 turn to f32 by adding them
+//   to the bits of 1.5 * 2^23. One or two column tiles: the planes' scales are
+//   applied to each. Three: the planes are joined first, in groups of 32 all in
+//   s32 (32 * 15 * 2^22 < 2^31), of more the two low ones in s32 (128 * 15 * 2^15
+//   < 2^26) and the high one in f32. Then the group's scale, and the sum of the
+//   row in f32.
 // - The inputs of a k32 step may be any 32 as long as both operands agree, so
 //   the packed layout gives thread c of a quad 8 consecutive codes (one
 //   word) of each group of 32, even codes in one register, odd ones in the
@@ -98,14 +100,18 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Whole sums of a group that the join of three column tiles takes off, by
+// groups in a block: of all planes together, or of the high one and of the others.
+constexpr int w4_sums(int gb) { return gb == 4 ? 1 : 2; }
+
 // Eight inputs of x row t into the planes' rows of shared memory (even ones,
 // then odd ones). The 16 threads of a half warp hold a block of 128. With it
-// the block's scales and the groups' sums: of each plane (three numbers each;
-// the sums are whole), or of the whole numbers (JOINT: one each, floats).
+// the block's scales and the groups' whole sums: of each plane (three numbers
+// each), or of planes together (JOINT: one scale, w4_sums sums `sum_next` apart).
 template <int GROUP, bool JOINT>
 __device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0, uint8_t* dst,
                                           int row_bytes, float* scale, float* sums,
-                                          int sum_stride) {
+                                          int sum_stride, int sum_next) {
   float f[8];
   const int64_t at = t * a.x_stride + k0;
   const char* src = static_cast<const char*>(a.x) + at * (a.dtype_x == kF32 ? 4 : 2);
@@ -152,9 +158,11 @@ __device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0
   auto unit = [&](int p) { return __uint_as_float((uint32_t)(e - 5 - 8 * p) << 23) + odd; };
   float* at_group = sums + lane / (GROUP / 8) * sum_stride;
   if constexpr (JOINT) {
-    if (lane % (GROUP / 8) == 0)
-      *at_group = GROUP == 32 ? __int_as_float(sum[0] * 65536 + sum[1] * 256 + sum[2])
-                              : fmaf((float)sum[0], 65536.f, fmaf((float)sum[1], 256.f, (float)sum[2]));
+    if (lane % (GROUP / 8) == 0) {
+      const int low = sum[1] * 256 + sum[2];
+      at_group[0] = __int_as_float(GROUP == 32 ? sum[0] * 65536 + low : sum[0]);
+      if (GROUP != 32) at_group[sum_next] = __int_as_float(low);
+    }
     if (lane == 0) *scale = unit(2);
   } else {
 #pragma unroll
@@ -167,8 +175,10 @@ __device__ __forceinline__ void w4_stage8(const W4Args& a, int64_t t, int64_t k0
 
 // More than eight rows of x are split once, by w4_planes_kernel, instead of in
 // every CTA. A (row, pair of blocks) in the workspace: the planes' 256 bytes
-// each, the blocks' two scales, the groups' 2 GB sums, to a multiple of 16 bytes.
-constexpr int w4_split_bytes(int gb) { return (kW4Planes * 256 + 2 * 4 * (1 + gb) + 15) / 16 * 16; }
+// each, the blocks' two scales, the 2 GB groups' sums, to a multiple of 16 bytes.
+constexpr int w4_split_bytes(int gb) {
+  return (kW4Planes * 256 + 2 * 4 * (1 + gb * w4_sums(gb)) + 15) / 16 * 16;
+}
 
 template <int GROUP>
 __global__ void __launch_bounds__(256) w4_planes_kernel(W4Args a) {
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(256) w4_planes_kernel(W4Args a) {
   float* scales = reinterpret_cast<float*>(out + kW4Planes * 256);
   w4_stage8<GROUP, true>(a, i / pairs, (i % pairs) * 256 + lane * 8,
                          out + blk * 128 + (e & 3) * 32 + (e >> 2) * 8, 256, scales + blk,
-                         scales + 2 + blk * GB, 1);
+                         scales + 2 + blk * GB * w4_sums(GB), w4_sums(GB), 1);
 }
 
 __device__ __forceinline__ float w4_scale(uint32_t bits, bool bf16) {
@@ -201,10 +211,11 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
   // planes of its two rows and joins them before it scales.
   constexpr bool JOINT = NT == 3;
   constexpr int XC = JOINT ? 8 : NT * 8;
-  // of a block's columns: scales [2 chunk][XC], a group's sums [2 chunk GB][XC]
+  constexpr int SUMS = JOINT ? w4_sums(GB) : 1;
+  // of a block's columns: scales [2 chunk][XC], a group's sums [2 chunk GB][SUMS][XC]
   float* xscale = part + (pl.split > 1 ? 2 * pl.mt * cta_rows : 0);
   float* xsum = xscale + 2 * pl.chunk * XC;
-  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + 2 * pl.chunk * GB * XC);  // what columns past the last read
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + 2 * pl.chunk * GB * SUMS * XC);  // what columns past the last read
   uint8_t* xs = zeros + 256;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, n = lane >> 2;
   const int wk = warp % pl.wk, wr = warp / pl.wk;
@@ -283,7 +294,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
 #pragma unroll
   for (int d = 0; d < kW4Ring; d++) fetch(d);
   fetch_meta(ahead);
-  for (int i = threadIdx.x; i < 2 * pl.chunk * XC * (1 + GB) + 64; i += THREADS)
+  for (int i = threadIdx.x; i < 2 * pl.chunk * XC * (1 + GB * SUMS) + 64; i += THREADS)
     xscale[i] = 0.f;  // and xsum, and zeros
   constexpr int kMagic = 0x4b400000;  // 1.5 * 2^23: adding |v| < 2^22 gives the float 1.5 * 2^23 + v
 
@@ -304,7 +315,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
         __syncthreads();  // what was staged before has been read
         const int eights = (end - ch) * 32;
         if (pl.split_x) {
-          constexpr int BYTES = w4_split_bytes(GB), FLOATS = 2 + 2 * GB;
+          constexpr int BYTES = w4_split_bytes(GB), FLOATS = 2 + 2 * GB * SUMS;
           const uint8_t* src = static_cast<const uint8_t*>(a.ws) + (m0 * pairs + ch) * BYTES;
           const int n_pairs = end - ch, words = P * 16;
           for (int i = threadIdx.x; i < mt * n_pairs * words; i += THREADS) {
@@ -316,7 +327,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
             const int j = i % FLOATS, q = i / FLOATS, t = q / n_pairs, pr = q % n_pairs;
             const float v = __ldg(reinterpret_cast<const float*>(src + ((int64_t)t * pairs + pr) * BYTES + P * 256) + j);
             if (j < 2) xscale[(pr * 2 + j) * XC + t] = v;
-            else xsum[(pr * 2 * GB + j - 2) * XC + t] = v;
+            else xsum[(pr * 2 * GB * SUMS + j - 2) * XC + t] = v;
           }
         } else {
           for (int i = threadIdx.x; i < eights * mt; i += THREADS) {
@@ -324,7 +335,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
             w4_stage8<GROUP, JOINT>(a, m0 + t, (int64_t)ch * 256 + e * 8,
                                     xs + column(t, 0) * row_bytes + (e >> 4) * 128 + (e & 3) * 32 + ((e >> 2) & 3) * 8,
                                     (JOINT ? 8 : 1) * row_bytes, &xscale[(e >> 4) * XC + at],
-                                    &xsum[(e >> 4) * GB * XC + at], XC);
+                                    &xsum[(e >> 4) * GB * SUMS * XC + at], SUMS * XC, XC);
           }
         }
         __syncthreads();
@@ -348,7 +359,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
         for (int t = 0; t < NT; t++)
           xb[t] = (has_column(t) ? xs + (8 * t + n) * row_bytes + (p - ch) * 256 : zeros) + c * 32;
         const float* bs = xscale + (p - ch) * 2 * XC + 2 * c;
-        const float* bz = xsum + (p - ch) * 2 * GB * XC + 2 * c;
+        const float* bz = xsum + (p - ch) * 2 * GB * SUMS * XC + 2 * c;
         // Two words of one block: 64 inputs of both m16 tiles.
         auto words = [&](int k, int i2, int (&sum)[2][NT][4]) {
           uint4 x[NT];
@@ -369,7 +380,7 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
               for (int t = 0; t < NT; t++) {
                 if (first)
 #pragma unroll
-                  for (int e = 0; e < 4; e++) sum[rt][t][e] = JOINT && GROUP == 32 ? 0 : kMagic;
+                  for (int e = 0; e < 4; e++) sum[rt][t][e] = JOINT && (GROUP == 32 || t > 0) ? 0 : kMagic;
                 mma_u8s8(sum[rt][t], f, h ? x[t].z : x[t].x, h ? x[t].w : x[t].y);
               }
             }
@@ -396,15 +407,14 @@ __global__ void __launch_bounds__(w4_warps(NT) * 32, w4_ctas(NT)) linear_w4_kern
                   }
                 } else if constexpr (JOINT) {
                   const float2 b2 = *reinterpret_cast<const float2*>(bs + k * XC);
-                  const float2 z2 = *reinterpret_cast<const float2*>(bz + g * XC);
+                  const int2 zh = *reinterpret_cast<const int2*>(bz + g * SUMS * XC);
+                  const int2 zl = *reinterpret_cast<const int2*>(bz + (g * SUMS + 1) * XC);
 #pragma unroll
                   for (int e = 0; e < 4; e++) {
-                    float v[3];
-#pragma unroll
-                    for (int q = 0; q < 3; q++) v[q] = __int_as_float(sum[rt][q][e]) - 12582912.f;
-                    const float whole = fmaf(v[0], 65536.f, fmaf(v[1], 256.f, v[2]));
-                    acc[rt][0][e] = fmaf(fmaf(-(float)z[e >> 1], e & 1 ? z2.y : z2.x, whole),
-                                         s[e >> 1] * (e & 1 ? b2.y : b2.x), acc[rt][0][e]);
+                    const int high = sum[rt][0][e] - z[e >> 1] * (e & 1 ? zh.y : zh.x);
+                    const int low = sum[rt][1][e] * 256 + sum[rt][2][e] - z[e >> 1] * (e & 1 ? zl.y : zl.x);
+                    const float whole = fmaf(__int_as_float(high) - 12582912.f, 65536.f, (float)low);
+                    acc[rt][0][e] = fmaf(whole, s[e >> 1] * (e & 1 ? b2.y : b2.x), acc[rt][0][e]);
                   }
                 } else {
 #pragma unroll
@@ -522,6 +532,7 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
   p.split_x = m > kW4Rows;
   p.nt = w4_column_tiles(m);
   const int cols = p.nt == 3 ? 24 : p.mt * kW4Planes, xc = p.nt == 3 ? 8 : 8 * p.nt;
+  const int floats = 1 + gb * (p.nt == 3 ? w4_sums(gb) : 1);  // of a block and column
   const int64_t tiles = (out_f + kW4Tile - 1) / kW4Tile, pairs = (in_f + 255) / 256;
   const int warps = w4_warps(p.nt);
   const int fixed = w4_ring_bytes(p.nt) + w4_red_bytes(p.nt);
@@ -532,7 +543,7 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
       const int part = split > 1 ? 2 * p.mt * wr * kW4Tile * 4 : 0;
       const int64_t range = (pairs + split - 1) / split;
       const int64_t left = w4_smem(p.nt) - fixed - part - 16 * cols - 256;
-      const int64_t fit = std::max<int64_t>(left, 0) / (256 * cols + 8 * xc * (1 + gb)) / wk * wk;
+      const int64_t fit = std::max<int64_t>(left, 0) / (256 * cols + 8 * xc * floats) / wk * wk;
       if (fit == 0) continue;  // chunks are whole turns of the wk warps
       const int64_t chunk = std::min(range, fit);
       const int64_t units = (tiles + wr - 1) / wr;
@@ -558,7 +569,7 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
         p.chunk = (int)chunk;
         p.units = (int)units;
         p.grid = (int)grid;
-        p.smem = fixed + part + (int)chunk * 8 * xc * (1 + gb) + 256 + cols * (int)(chunk * 256 + 16);
+        p.smem = fixed + part + (int)chunk * 8 * xc * floats + 256 + cols * (int)(chunk * 256 + 16);
       }
     }
   return p;

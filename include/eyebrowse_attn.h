@@ -371,8 +371,10 @@ EB_API int eb_w4_quantize(const float* w, int64_t in_f, int64_t out_f, int32_t g
  * or bf16, rows x_stride / y_stride elements apart (0 = in_f / out_f); x and y
  * do not overlap. An activation enters as a whole number of units of a power
  * of two, with an error of at most 2^-22 of the largest of its block of 128
- * neighbouring inputs; sums are of whole numbers within a group and in f32
- * beyond. A row with a value that is not finite yields NaN. Made for the few rows of decode steps: up to 8 rows stream the
+ * neighbouring inputs (or 2^-122, if that is more); a group's sum, its zero
+ * point's share taken off, is of whole numbers, and rounded to f32 once; sums
+ * beyond are in f32. A row with a value that is not finite yields NaN in every
+ * output. Made for the few rows of decode steps: up to 8 rows stream the
  * weights once, more rows once more for each 8 (from L2 where they fit).
  * m <= 2^18, in_f and out_f <= 2^24. eb_linear_w4_workspace_bytes is 0 for
  * m <= 8; above, the rows' whole numbers lie there. The workspace is 256-byte
