@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kSampleThreads, 3) sample_kernel(SampleArgs a)
   const bool greedy = !(temp > 0.f);
   const int top_k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.f;
-  const double min_p = a.min_p && a.min_p[r] > 0.f ? (double)a.min_p[r] : 0.0;
+  // past 1 nothing would be kept: as 1, the largest logit and its equals are
+  const double min_p = a.min_p && a.min_p[r] > 0.f ? (double)fminf(a.min_p[r], 1.f) : 0.0;
   const bool k_on = !greedy && top_k > 0 && top_k < n, p_on = !greedy && top_p < 1.f;
   // One variable decides which passes a row takes. (With the conditions
   // spelled out at each branch nvcc 12.9 dropped the one before pass 2.)

@@ -450,7 +450,7 @@ typedef struct {
   const float* temperature; /* <= 0 or NaN: greedy, the largest logit, the first of equals */
   const int32_t* top_k;     /* < 1: off */
   const float* top_p;       /* >= 1 or NaN: off; <= 0: one token */
-  const float* min_p;       /* <= 0 or NaN: off */
+  const float* min_p;       /* <= 0 or NaN: off; > 1: as 1 */
 } eb_sample_params;
 
 /* One token id per row of logits [rows, vocab] (f32, f16 or bf16, rows
@@ -460,7 +460,8 @@ typedef struct {
  *   top_k keeps the first top_k tokens;
  *   top_p keeps, of those, each token before which less than top_p of their
  *   weight stands (so at least one);
- *   min_p keeps, of those, the weights of at least min_p, and the largest.
+ *   min_p keeps, of those, the weights of at least min_p (past 1 it counts as 1:
+ *   the largest logit's equals stay).
  * The id is the first, in the vocabulary's order, at which the running sum of
  * the kept weights passes u times their total. Weights and sums are in f64,
  * so that the draw does not hang on rounding; results do not depend on
