@@ -952,7 +952,8 @@ static int kv8_check(const eb_attn_desc* d, const eb_attn_layer* L, const eb_kv8
   if (d->dtype_cache != EB_E4M3 && d->dtype_cache != EB_E5M2) return EB_ERR_INVALID_ARGUMENT;
   eb_attn_desc t = *d;
   t.dtype_cache = EB_F32;  // the other fields are checked as everywhere
-  if (!desc_ok(&t) || d->n_kv_heads > 65535) return EB_ERR_INVALID_ARGUMENT;
+  // (the kernels step over rows in 32 bits)
+  if (!desc_ok(&t) || d->n_kv_heads > 65535 || d->max_seq > (1 << 30)) return EB_ERR_INVALID_ARGUMENT;
   if (L && (L->rope_cos == nullptr) != (L->rope_sin == nullptr)) return EB_ERR_INVALID_ARGUMENT;
   if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
     return EB_ERR_INVALID_ARGUMENT;

@@ -388,7 +388,8 @@ EB_API int eb_linear_w4(const eb_w4* w, const void* x, int32_t dtype_x, int64_t 
 /* An 8-bit KV cache: codes in desc->dtype_cache (EB_E4M3 or EB_E5M2) and one
  * f32 scale per (block of rows, KV head), for K and for V; the value of a
  * code is code * scale.
- *   k, v:             [max_seq, n_kv_heads, head_dim] bytes, 16-byte aligned
+ *   k, v:             [max_seq, n_kv_heads, head_dim] bytes, 16-byte aligned;
+ *                     max_seq <= 2^30
  *   k_scale, v_scale: [ceil(max_seq / block), n_kv_heads] f32
  * Calls that write choose the scale: the smallest power of two (2^-64 at
  * least) at which no finite value of the new rows passes the type's largest
