@@ -77,6 +77,13 @@ class W4(ctypes.Structure):
 
 class Kv8(ctypes.Structure):
     """eb_kv8: an 8-bit KV cache with block scales."""
+    codes = scales = 1 << 62  # elements from the first on that k and v, and their scales, hold
+    dims = None               # (max_seq, kv_heads, head_dim) where the tensors have these axes
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.plans = {}  # what calls expect of their tensors, by descriptor and batch
+
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
                 ("v_scale", ctypes.c_void_p), ("batch_stride", ctypes.c_int64),
                 ("scale_batch_stride", ctypes.c_int64), ("block", ctypes.c_int32)]
@@ -172,18 +179,18 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-_torch = None  # torch, once a call has needed it
+_raw_stream = _device = None  # torch's, once a call has needed them
 
 
 def _stream(stream) -> int | None:
-    global _torch
+    global _raw_stream, _device
     if stream is None:
-        if _torch is None:
+        if _raw_stream is None:
             import torch
             torch.cuda.init()
-            _torch = torch
+            _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
         # torch.cuda.current_stream() without the Stream object around it
-        return _torch._C._cuda_getCurrentRawStream(_torch._C._cuda_getDevice())
+        return _raw_stream(_device())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -197,11 +204,15 @@ def _check(status: int, what: str) -> None:
 _dtype_codes = {}
 
 
-def torch_dtype_code(dt) -> int:
+def _codes() -> dict:
     if not _dtype_codes:
         import torch
         _dtype_codes.update({torch.float32: EB_F32, torch.float16: EB_F16, torch.bfloat16: EB_BF16})
-    return _dtype_codes[dt]
+    return _dtype_codes
+
+
+def torch_dtype_code(dt) -> int:
+    return _codes()[dt]
 
 
 # ---------------------------------------------------------------- kernel level
@@ -291,12 +302,24 @@ def w4_quantize(w, group=128, zero_point=False, dtype_scale=EB_F16):
 
 
 def make_w4(q, scale, zero, in_f, out_f, group, dtype_scale=None):
-    """eb_w4 over device tensors (kept alive by the object). The scale type is the scale
-    tensor's unless dtype_scale says otherwise."""
+    """eb_w4 over dense device tensors (kept alive by the object): q as w4_pack lays it out, scale
+    (2 bytes an element) and zero [ceil(in_f / group), out_f]. The scale type is the scale tensor's
+    unless dtype_scale says otherwise."""
     _dtype(q, "u8", "make_w4: q")
     _dtype(zero, "u8", "make_w4: zero")
     if dtype_scale is None:
         dtype_scale = torch_dtype_code(scale.dtype)
+    if hasattr(scale, "element_size") and scale.element_size() != 2:
+        _refuse(f"make_w4: scales of {scale.dtype}")
+    groups = -(-in_f // group) if group > 0 else 0
+    for t, n, name in ((q, w4_weight_bytes(in_f, out_f), "q"), (scale, groups * out_f, "scale"),
+                       (zero, groups * out_f, "zero")):
+        if hasattr(t, "numel") and not (t.is_contiguous() and t.numel() >= n):
+            _refuse(f"make_w4: {name} of shape {tuple(t.shape)}, strides {t.stride()}, for {in_f} inputs and "
+                    f"{out_f} outputs in groups of {group}")
+    for name, t in (("scale", scale), ("zero", zero)):
+        if getattr(t, "ndim", 0) == 2 and groups and tuple(t.shape) != (groups, out_f):
+            _refuse(f"make_w4: {name} of shape {tuple(t.shape)}, not {(groups, out_f)}")
     w = W4(in_f, out_f, group, dtype_scale, _ptr(q), _ptr(scale), _ptr(zero))
     w._keepalive = (q, scale, zero)
     return w
@@ -493,21 +516,99 @@ def attention_decode_noalloc(desc, layer, pos, q, k, v, kcache, vcache, o, strea
 
 
 # ---------------------------------------------------------------- 8-bit cache
+def _batches(a, b, inner, stride, what):
+    """Elements that two tensors of one layout hold from their first on, and the stride between
+    sequences: `stride`, or what their leading axis (in front of `inner` others) has if it is not
+    dense. Sequences are dense in themselves."""
+    if a.shape != b.shape or a.stride() != b.stride():
+        _refuse(f"{what}: shapes {tuple(a.shape)} and {tuple(b.shape)}, strides {a.stride()} and {b.stride()}")
+    if a.is_contiguous():
+        return a.numel(), stride
+    st = a.stride()
+    if a.ndim != inner + 1 or a.numel() == 0 or not a[0].is_contiguous() or st[0] < a[0].numel() or (stride and stride != st[0]):
+        _refuse(f"{what}: shape {tuple(a.shape)}, strides {st}")
+    return (a.shape[0] - 1) * st[0] + a[0].numel(), st[0]
+
+
 def make_kv8(k, v, k_scale, v_scale, block, batch_stride=0, scale_batch_stride=0):
     """eb_kv8 over device tensors (kept alive by the object): codes [(batch,) max_seq, kv_heads,
-    head_dim] of one byte, scales f32 [(batch,) ceil(max_seq / block), kv_heads]."""
+    head_dim] of one byte, scales f32 [(batch,) ceil(max_seq / block), kv_heads]. Sequences may lie
+    apart, as a slice of a longer cache has them."""
     for t, name in ((k, "u8"), (v, "u8"), (k_scale, "float32"), (v_scale, "float32")):
         _dtype(t, name, "make_kv8")
+    tensors = hasattr(k, "numel") and hasattr(v, "numel")
+    if tensors:
+        codes, batch_stride = _batches(k, v, 3, batch_stride, "make_kv8")
+    if hasattr(k_scale, "numel") and hasattr(v_scale, "numel"):
+        scales, scale_batch_stride = _batches(k_scale, v_scale, 2, scale_batch_stride, "make_kv8: scales")
     c = Kv8(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), batch_stride, scale_batch_stride, block)
+    if tensors:
+        c.codes = codes
+        if k.ndim >= 3:
+            c.dims = tuple(k.shape[-3:])
+    if hasattr(k_scale, "numel") and hasattr(v_scale, "numel"):
+        c.scales = scales
     c._keepalive = (k, v, k_scale, v_scale)
     return c
+
+
+def _kv8_plan(desc, c, batch, what):
+    """What a call over `batch` sequences as desc describes them expects of its tensors: types, widths
+    and strides of the rows, once per descriptor and batch. A cache that does not hold the
+    sequences is refused."""
+    key = bytes(desc), batch
+    plan = c.plans.get(key)
+    if plan:
+        return plan
+    rows, heads, hd = desc.max_seq, desc.n_kv_heads, desc.head_dim
+    if c.dims is not None and (c.dims[1] != heads or c.dims[2] != hd or rows > c.dims[0]
+                               or (batch > 1 and rows != c.dims[0] and not c.batch_stride)):
+        _refuse(f"{what}: a cache of {c.dims} for {rows} rows of {heads} heads of {hd}")
+    n, s = rows * heads * hd, -(-rows // max(1, c.block)) * heads
+    if (n + ((batch - 1) * (c.batch_stride or n) if batch > 1 else 0) > c.codes
+            or s + ((batch - 1) * (c.scale_batch_stride or s) if batch > 1 else 0) > c.scales):
+        _refuse(f"{what}: a cache of {c.codes} codes and {c.scales} scales")
+    q, kv = desc.n_heads * hd, heads * hd
+    types = {code: dt for dt, code in _codes().items()}
+    plan = (types.get(desc.dtype_qkv), types.get(desc.dtype_out), q, desc.q_stride or q, kv, desc.kv_stride or kv,
+            desc.o_stride or q)
+    if len(c.plans) >= 64:
+        c.plans.clear()
+    c.plans[key] = plan
+    return plan
+
+
+def _rows(t, dtype, rows, width, stride, what):
+    """Pointer of a tensor that holds `rows` rows of `width` elements, `stride` apart; others are
+    refused. Pointers and None pass as they are."""
+    try:
+        have = t.dtype
+    except AttributeError:
+        return _ptr(t)
+    if have is dtype and t.numel() == rows * width and (stride == width or rows == 1) and t.is_contiguous():
+        return t.data_ptr()
+    shape, st = t.shape, t.stride()
+    if have is dtype:
+        if len(shape) == 2 and st[1] == 1 and shape[1] >= width and shape[0] >= rows and (st[0] == stride or rows == 1):
+            return t.data_ptr()
+        if (len(shape) > 1 and shape[0] >= rows and (st[0] == stride or rows == 1) and t[0].is_contiguous()
+                and t[0].numel() >= width):
+            return t.data_ptr()
+        # one run of elements, without an axis for the rows
+        if (rows == 1 or len(shape) == 1) and t.is_contiguous() and t.numel() >= (rows - 1) * stride + width:
+            return t.data_ptr()
+    _refuse(f"{what}: {have}, shape {tuple(shape)}, strides {st} for {rows} rows of {width}, {stride} apart, in {dtype}")
 
 
 def kv8_write(desc, layer, cache: Kv8, start, count, k, v, stream=None):
     """eb_kv8_write: rows [start, start + count) of one sequence's 8-bit cache; layer None writes
     the rows as they are."""
-    _check(lib().eb_kv8_write(desc, layer, cache, start, count, _ptr(k), _ptr(v),
-                              _stream(stream)), "eb_kv8_write")
+    dt, _, _, _, width, stride, _ = (cache.plans.get((bytes(desc), 1))
+                                     or _kv8_plan(desc, cache, 1, "kv8_write"))
+    _check((_lib or lib()).eb_kv8_write(desc, layer, cache, start, count,
+                                        _rows(k, dt, count, width, stride, "kv8_write: k"),
+                                        _rows(v, dt, count, width, stride, "kv8_write: v"), _stream(stream)),
+           "eb_kv8_write")
 
 
 def attention_decode_kv8_workspace_bytes(desc, batch, max_pos) -> int:
@@ -518,10 +619,17 @@ def attention_decode_kv8(desc, layer, cache: Kv8, batch, positions, max_pos, q, 
                          workspace=None, stream=None):
     """eb_attention_decode_kv8: one decode step per sequence over an 8-bit cache; positions None
     puts every sequence at max_pos, k and v None append nothing."""
+    what = "attention_decode_kv8"
+    dt, dt_o, nq, sq, nkv, skv, so = _kv8_plan(desc, cache, batch, what)
+    if hasattr(positions, "numel"):
+        _dtype(positions, "int32", what)
+        if positions.numel() < batch or not positions.is_contiguous():
+            _refuse(f"{what}: {positions.numel()} positions for {batch} sequences, or strided")
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _check(lib().eb_attention_decode_kv8(desc, layer, cache, batch, _ptr(positions), max_pos,
-                                         _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(workspace),
-                                         ws_bytes, _stream(stream)), "eb_attention_decode_kv8")
+                                         _rows(q, dt, batch, nq, sq, what), _rows(k, dt, batch, nkv, skv, what),
+                                         _rows(v, dt, batch, nkv, skv, what), _rows(o, dt_o, batch, nq, so, what),
+                                         _ptr(workspace), ws_bytes, _stream(stream)), "eb_attention_decode_kv8")
 
 
 # ---------------------------------------------------------------- sampling
