@@ -274,10 +274,13 @@ def w4_weight_bytes(in_f, out_f) -> int:
 
 
 def w4_pack(codes):
-    """eb_w4_pack (host): codes [out_f, in_f] (numpy uint8, 0..15) -> packed uint8 rows
+    """eb_w4_pack (host): codes [out_f, in_f] (numpy, 0..15) -> packed uint8 rows
     [out_f, ceil(in_f / 128) * 64]."""
     import numpy as np
-    codes = np.ascontiguousarray(codes, dtype=np.uint8)
+    given = np.asarray(codes)
+    codes = np.ascontiguousarray(given, dtype=np.uint8)
+    if given.dtype != np.uint8 and not np.array_equal(codes, given):
+        _refuse("w4_pack: codes that are not whole numbers of 0..15")
     out_f, in_f = codes.shape
     q = np.empty((out_f, (in_f + 127) // 128 * 64), np.uint8)
     _check(lib().eb_w4_pack(codes.ctypes.data, in_f, out_f, q.ctypes.data), "eb_w4_pack")

@@ -130,3 +130,15 @@ def test_kv8_rows_the_kernels_would_misread(eb):
     for kw in (dict(k=k.half()), dict(v=k.half()), dict(k=k[:1]), dict(v=k[:, :127]), dict(k=fused[:, :128]), dict(k=fused),
                dict(d=strided), dict(k=fused[:, ::4]), dict(count=3), dict(k=t(128, 2).t()), dict(k=t(255))):
         _refused(eb, write, **kw)
+
+
+def test_w4_pack_takes_codes_as_they_are(eb):
+    """Codes past a byte are refused as those past 15 are, not wrapped into its range."""
+    import numpy as np
+    ok = np.arange(16)[None]
+    assert np.array_equal(eb.w4_pack(ok), eb.w4_pack(ok.astype(np.uint8)))
+    for bad in (256, 261, -251, 16, -1):
+        codes = ok.copy()
+        codes[0, 3] = bad
+        _refused(eb, eb.w4_pack, codes)
+    _refused(eb, eb.w4_pack, ok + 0.5)
