@@ -229,7 +229,7 @@ struct Kv8DecodeArgs {
 };
 // Any even head_dim up to 256.
 cudaError_t launch_kv8_decode(const Kv8DecodeArgs& a, cudaStream_t st);
-// head_dim 128 and 256 (eb_kv8_tc.cu).
+// head_dim 64, 128 and 256 (eb_kv8_tc.cu).
 bool kv8_tc_supported(int hd);
 cudaError_t launch_kv8_decode_tc(const Kv8DecodeArgs& a, cudaStream_t st);
 

@@ -398,9 +398,12 @@ EB_API int eb_linear_w4(const eb_w4* w, const void* x, int32_t dtype_x, int64_t 
  * smaller scale they are rounded again at the new one, which is exact but
  * for values that become subnormal. A write of a block's first row starts
  * the block anew, whatever it held. Values round to nearest, ties to even;
- * an infinity is stored as the type's largest value, a NaN as NaN. Rows
- * behind the written ones are left as they are. Calls that only read take
- * any positive scales. */
+ * an infinity is stored as the type's largest value, a NaN as NaN. Codes of
+ * rows behind the written ones are left as they are (rows of a block whose
+ * scale grew then stand for larger values: they are to be written again).
+ * Calls that read take any positive K scale, and V scales of 2^-64 to 2^95:
+ * at head_dim 64, 128 and 256 the softmax weights lose a bit for each power of
+ * two beyond. */
 typedef struct {
   void* k;
   void* v;
@@ -426,10 +429,10 @@ EB_API int eb_kv8_write(const eb_attn_desc* desc, const eb_attn_layer* layer, co
  * rows 0..=positions[b] (the last `window` of them) into o. Scores, softmax
  * statistics and sums are in f32; at head_dim 64, 128 and 256 q and the
  * weights enter the products with 20 bits where o is f32 and with 16 where o
- * is a 16-bit type, else in f32. batch <= 32767. positions: DEVICE int32; a
- * value outside [0,
- * max_pos] marks an empty slot of the batch, whose cache and output rows are
- * left as they are. positions == NULL: every sequence is at max_pos. No two
+ * is a 16-bit type (a weight to within 2^-31 or 2^-27 of the largest at
+ * least), else in f32. batch <= 32767. positions: DEVICE int32; a value
+ * outside [0, max_pos] marks an empty slot of the batch, whose cache and output
+ * rows are left as they are. positions == NULL: every sequence is at max_pos. No two
  * sequences of a call share rows that it writes. Row strides as for
  * eb_attention_decode_batched; no alignment beyond the element's for q, k, v
  * and o. A workspace smaller than
