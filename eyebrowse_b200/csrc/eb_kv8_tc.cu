@@ -37,11 +37,13 @@
 // spin-wait).
 //
 // Measured: 64 sequences of 512 to 16384 rows, 8 KV heads of 128 with four query
-// heads each, 196 to 206 us, of which HBM needs 165: it is
-// bound by the softmax threads, four exponentials and four splits of a weight
-// into planes for each 256 bytes a row has. One sequence of 2048 rows 12 us: the
-// launch, the append, one trip to HBM, four barriers a tile and the merge.
-// head_dim 64: 64 sequences of 8192 rows, 8 KV heads, 124 us (the bytes need 82).
+// heads each, 196 to 207 us, of which HBM needs 165: it is bound by the softmax
+// threads, four exponentials and four splits of a weight into planes for each
+// 256 bytes a row has. One sequence of 2048 rows 12 us: the
+// launch, the append, one trip to HBM, four barriers a tile and the merge. At
+// head_dim 256 the ring (192 KB) leaves one CTA an SM: 24 sequences with a window
+// of 1024, 4 KV heads, 28.5 us, 192 CTAs in 148 places. head_dim 64: 64
+// sequences of 8192 rows, 8 KV heads, 124 us (the bytes need 82).
 #include "eb_kv8.cuh"
 #include "eb_rowops.cuh"
 #include "eb_tc.cuh"

@@ -29,8 +29,12 @@
 // the sort).
 //
 // A row is shared by a cluster of 1 to 16 CTAs; passes after the first read it
-// from L1 or L2. What bounds it: for many open rows the f64 pipe (12
-// operations a token), for one row the chain of cluster barriers.
+// from L1 or L2. What bounds it: for one row the chain of five cluster barriers
+// (of ten where the quick bound fails) with rank 0 alone at work in between; for
+// many rows latency, at 24 warps an SM of 80 registers (and some spills): 256 open
+// rows take 98 us, of which the f64 pipe needs 22 (12 operations a token), with
+// 512 CTAs in 444 places. A bisection is far slower: rows of 151936 take 0.23 to
+// 0.53 ms alone, 64 of them 0.8 to 1.9 ms.
 #include <cooperative_groups.h>
 
 #include <algorithm>

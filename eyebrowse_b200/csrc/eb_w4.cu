@@ -22,7 +22,7 @@ namespace eb {
 // m16n8k32, u8 codes by s8 activations, s32 sums. At a few rows of x the work is
 // a stream of the weights, and what a warp does per code, not the matrix rate,
 // has to keep under its share of the memory bandwidth (about 2.5 instruction
-// slots per code and lane at 6.5 TB/s). Eight codes in a word become two
+// slots per code and lane at 6.5 TB/s; one row takes 1.9). Eight codes in a word become two
 // operand registers with a shift and two ANDs; f16 operands took eleven
 // instructions (and twice the MMAs: both kinds issue at one per two clocks and
 // SM here, with k16 and k32). A tcgen05 operand would have to pass through
@@ -53,11 +53,14 @@ namespace eb {
 //
 // Measured (calls in a row, weights from HBM; in brackets from L2 and out of a
 // graph, and there with f16 operands): one row by 4096 x 28672 22.5 us (16.5,
-// 26), eight rows by 14336 x 4096 27 us (23.5, 39), 37 rows by 4100 x 5003 in
-// groups of 32 45 us (41, 52; joined in f32 49), one row by 1024 x 4096 6.7 us (4.6, 4.8), which is
-// a launch, one trip to memory and the sums' two meetings. The large ones are
-// bound by issue slots: unpacking, and with eight rows the groups' sums (eight
-// f32 operations per output, group and plane triple).
+// 26), eight rows by 14336 x 4096 26.6 us (23.5, 39), 37 rows by 4100 x 5003 in
+// groups of 32 45 us (41, 52; joined in f32 49), one row by 1024 x 4096 6.6 us
+// (4.6, 4.8), which is a launch, one trip to memory and the sums' two meetings.
+// The large ones are bound by latency: 12 to 16 warps an SM (115 to 128
+// registers a thread), each a chain of wait, unpack, products and join; an
+// instruction is issued in 35 % (one row) to 49 % (37 rows) of the clocks in which
+// an SM has work, and the grids leave a part of the SMs empty or half empty (224
+// of 296 places, 128 and 125 of 148).
 constexpr int kW4Ring = 2;   // pairs of blocks of a warp in its ring of shared memory
 constexpr int kW4Pair = 4096;  // bytes of a tile's pair of blocks
 constexpr int kW4Tile = 32;  // weight rows of a warp: two m16 tiles
@@ -575,13 +578,19 @@ static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int*
   return p;
 }
 
-// Resident clusters of every size, asked of the runtime once per kernel.
+// Resident clusters of every size, asked of the runtime once per kernel and
+// device.
 template <int NT, int GROUP>
 static cudaError_t w4_limits(int (&limit)[9]) {
-  static int cache[9] = {};
+  static int cache[64][9] = {};
   auto kern = linear_w4_kernel<NT, GROUP>;
+  int dev = 0;
+  const cudaError_t have = cudaGetDevice(&dev);
+  if (have != cudaSuccess) return have;
+  int none[9] = {};
+  int* known = dev < 64 ? cache[dev] : none;
   for (int split = 1; split <= 8; split++) {
-    limit[split] = __atomic_load_n(&cache[split], __ATOMIC_RELAXED);
+    limit[split] = __atomic_load_n(&known[split], __ATOMIC_RELAXED);
     if (limit[split] > 0) continue;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(split);
@@ -596,7 +605,7 @@ static cudaError_t w4_limits(int (&limit)[9]) {
     const cudaError_t e = cudaOccupancyMaxActiveClusters(&limit[split], kern, &cfg);
     if (e != cudaSuccess) return e;
     if (limit[split] < 1) limit[split] = 1;
-    __atomic_store_n(&cache[split], limit[split], __ATOMIC_RELAXED);
+    __atomic_store_n(&known[split], limit[split], __ATOMIC_RELAXED);
   }
   return cudaSuccess;
 }

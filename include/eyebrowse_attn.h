@@ -375,7 +375,9 @@ EB_API int eb_w4_quantize(const float* w, int64_t in_f, int64_t out_f, int32_t g
  * point's share taken off, is of whole numbers, and rounded to f32 once; sums
  * beyond are in f32. A row with a value that is not finite yields NaN in every
  * output. Made for the few rows of decode steps: up to 8 rows stream the
- * weights once, more rows once more for each 8 (from L2 where they fit).
+ * weights once, more rows once more for each 8 (from L2 where they fit):
+ * hundreds of rows take several times as long as eb_linear_f16w (2048 rows of
+ * 14336 -> 4096: 2.4 ms against 0.41; 64 rows 84 us against 148).
  * m <= 2^18, in_f and out_f <= 2^24. eb_linear_w4_workspace_bytes is 0 for
  * m <= 8; above, the rows' whole numbers lie there. The workspace is 256-byte
  * aligned and needs no initialisation; calls that share one must not overlap
@@ -473,6 +475,10 @@ typedef struct {
  * drawn. A NaN logit counts as -infinity, several +infinity as equals that
  * leave no weight to others. A row without a logit above -infinity gives -1.
  * u is clamped to [0, 1 - 2^-24], NaN to 0.
+ * Where the cut falls among more than 2048 tokens of nearly equal weight (flat
+ * logits, a high temperature), or top_k passes 2048 beside a top_p, a row is
+ * passed over once or twice per bit of a key: 0.23 to 0.53 ms for one row of
+ * 151936, where others take 13 to 90 us.
  * ids: DEVICE int32 [rows]. rows and vocab <= 2^24. A row's scratch is in
  * shared memory: eb_sample_workspace_bytes is 0 and the workspace may be
  * NULL. */
