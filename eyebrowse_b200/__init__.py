@@ -78,7 +78,7 @@ class W4(ctypes.Structure):
 class Kv8(ctypes.Structure):
     """eb_kv8: an 8-bit KV cache with block scales."""
     codes = scales = 1 << 62  # elements from the first on that k and v, and their scales, hold
-    dims = None               # (max_seq, kv_heads, head_dim) where the tensors have these axes
+    axes = scale_axes = None  # the tensors' own: [(batch,) rows, kv_heads, head_dim], [(batch,) blocks, kv_heads]
 
     def __init__(self, *args, **kw):
         super().__init__(*args, **kw)
@@ -546,11 +546,9 @@ def make_kv8(k, v, k_scale, v_scale, block, batch_stride=0, scale_batch_stride=0
         scales, scale_batch_stride = _batches(k_scale, v_scale, 2, scale_batch_stride, "make_kv8: scales")
     c = Kv8(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), batch_stride, scale_batch_stride, block)
     if tensors:
-        c.codes = codes
-        if k.ndim >= 3:
-            c.dims = tuple(k.shape[-3:])
+        c.codes, c.axes = codes, tuple(k.shape)
     if hasattr(k_scale, "numel") and hasattr(v_scale, "numel"):
-        c.scales = scales
+        c.scales, c.scale_axes = scales, tuple(k_scale.shape)
     c._keepalive = (k, v, k_scale, v_scale)
     return c
 
@@ -564,10 +562,16 @@ def _kv8_plan(desc, c, batch, what):
     if plan:
         return plan
     rows, heads, hd = desc.max_seq, desc.n_kv_heads, desc.head_dim
-    if c.dims is not None and (c.dims[1] != heads or c.dims[2] != hd or rows > c.dims[0]
-                               or (batch > 1 and rows != c.dims[0] and not c.batch_stride)):
-        _refuse(f"{what}: a cache of {c.dims} for {rows} rows of {heads} heads of {hd}")
-    n, s = rows * heads * hd, -(-rows // max(1, c.block)) * heads
+    blocks = -(-rows // max(1, c.block))
+    # tensors with an axis for the sequences, for the rows or blocks, and for the rest
+    for have, want, stride in ((c.axes, (rows, heads, hd), c.batch_stride),
+                               (c.scale_axes, (blocks, heads), c.scale_batch_stride)):
+        if have is None or len(have) < len(want):
+            continue
+        own = have[-len(want):]
+        if own[1:] != want[1:] or own[0] < want[0] or (batch > 1 and len(have) > len(want) and own[0] != want[0] and not stride):
+            _refuse(f"{what}: a cache of {have}, {want} a sequence in the descriptor")
+    n, s = rows * heads * hd, blocks * heads
     if (n + ((batch - 1) * (c.batch_stride or n) if batch > 1 else 0) > c.codes
             or s + ((batch - 1) * (c.scale_batch_stride or s) if batch > 1 else 0) > c.scales):
         _refuse(f"{what}: a cache of {c.codes} codes and {c.scales} scales")

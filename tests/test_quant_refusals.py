@@ -86,6 +86,13 @@ def test_kv8_caches_smaller_than_the_descriptor_are_refused(eb):
         _refused(eb, write, c)
     _refused(eb, decode, _cache(eb, B=1))
     _refused(eb, decode, _cache(eb, S=100))  # dense sequences of 100 rows, read as of 96
+    longer, few = _cache(eb, S=130)._keepalive[2:], _cache(eb, h=3)._keepalive[2:]
+    for scales in (longer, few):             # five blocks a sequence, read as three; three heads, as two
+        _refused(eb, decode, _cache(eb, make=lambda t: t[:2] + list(scales)))  # noqa: B023
+    write(_cache(eb, make=lambda t: t[:2] + list(longer)))
+    both = _cache(eb, make=lambda t: [x.flatten(0, 1) for x in t])  # no axis for the sequences: dense
+    eb.attention_decode_kv8(_desc(eb), None, both, 0, None, 95, q, k, k, o, None, 0)
+    eb._kv8_plan(_desc(eb), both, 2, "dense")
     write(_cache(eb, S=100))                 # one sequence: the first 96 of its rows
     write(_cache(eb, make=lambda t: [x.flatten() for x in t[:2]] + t[2:]))
 
