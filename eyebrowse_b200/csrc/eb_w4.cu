@@ -526,7 +526,11 @@ size_t linear_w4_workspace_bytes(int64_t m, int64_t in_f, int64_t) {
 // what the longest row of pairs of one warp takes (a warp alone takes about as
 // long for a pair as a full SM for 16). limit[split]: clusters of that size that
 // are resident at once (an SM group holds whole clusters only: 148 SMs do not
-// hold 21 clusters of 7).
+// hold 21 clusters of 7). Measured against every other shape that fits (16 to 40
+// each) at nine sizes of 1 to 64 rows, 1024 -> 4096 to 4096 -> 28672: within 5 % of
+// the fastest (one row 4096 -> 28672 20.3 us, best 20.1, worst 78; eight rows
+// 14336 -> 4096 26.1, best 26.1, worst 175; 37 rows 4100 -> 5003 41.5, best 41.4,
+// worst 120).
 static W4Plan plan_w4(int64_t m, int64_t in_f, int64_t out_f, int gb, const int* limit) {
   W4Plan p{};
   const int sms = sm_count();
