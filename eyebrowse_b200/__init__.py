@@ -79,14 +79,13 @@ class Kv8(ctypes.Structure):
     """eb_kv8: an 8-bit KV cache with block scales."""
     codes = scales = 1 << 62  # elements from the first on that k and v, and their scales, hold
     axes = scale_axes = None  # the tensors' own: [(batch,) rows, kv_heads, head_dim], [(batch,) blocks, kv_heads]
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("batch_stride", ctypes.c_int64),
+                ("scale_batch_stride", ctypes.c_int64), ("block", ctypes.c_int32)]
 
     def __init__(self, *args, **kw):
         super().__init__(*args, **kw)
         self.plans = {}  # what calls expect of their tensors, by descriptor and batch
-
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
-                ("v_scale", ctypes.c_void_p), ("batch_stride", ctypes.c_int64),
-                ("scale_batch_stride", ctypes.c_int64), ("block", ctypes.c_int32)]
 
 
 class SampleParams(ctypes.Structure):
